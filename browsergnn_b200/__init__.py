@@ -17,6 +17,8 @@ host-side mirror of the reference's API for that path:
   LearningPathRecommender,
   ConceptPrerequisiteMapper                     src/models/*.ts
   serializeModel, loadModelFromJSON, ...        src/utils/serialization.ts
+  rmsNorm, gatedLinear, linearFused, logProbs
+  and their ...Backward                         (mixed precision, no counterpart)
 """
 from ._lib import BGNNError, BGNNIndexError
 from .backend import (CudaComputeManager, get_backend, get_compute_manager, get_context,
@@ -30,7 +32,11 @@ from .ops import (GPUSparse, GPUTensor, MessagePassing, SparseCOO, SparseCSR, co
 from .nn import (GELU, Dropout, Linear, LogSoftmax, PReLU, SiLU, Sigmoid, Softmax, Tanh,
                  manual_seed)
 from .models import ConceptPrerequisiteMapper, LearningPathRecommender, StudentMasteryPredictor
-from . import serialization
+from . import blocks, serialization
+from .blocks import (gated_linear, gated_linear_backward, gatedLinear, gatedLinearBackward,
+                     linear_fused, linear_fused_backward, linearFused, linearFusedBackward,
+                     log_probs, log_probs_backward, logProbs, logProbsBackward, rms_norm,
+                     rms_norm_backward, rmsNorm, rmsNormBackward)
 from .graphs import CapturedForward
 from .serialization import (deserializeModel, getModelSize, getStateDict, loadModelFromJSON,
                             loadStateDict, saveModelToJSON, serializeModel)
@@ -47,5 +53,5 @@ __all__ = [
     "manual_seed", "StudentMasteryPredictor", "LearningPathRecommender",
     "ConceptPrerequisiteMapper", "serialization", "serializeModel", "deserializeModel",
     "saveModelToJSON", "loadModelFromJSON", "getStateDict", "loadStateDict", "getModelSize",
-    "CapturedForward",
+    "CapturedForward", *blocks.__all__, "blocks",
 ]

@@ -20,6 +20,8 @@ AGGR = {"sum": 0, "add": 0, "mean": 1, "max": 2}
 AGGR_SPMM = 3
 ACT = {None: 0, "none": 0, "relu": 1, "relu_max": 2, "elu": 3, "leaky_relu": 4, "sigmoid": 5,
        "tanh": 6, "gelu": 7, "silu": 8}
+# bgnn_dtype
+F32, BF16, F16, E4M3 = range(4)
 LINK = {"dot": 0, "bilinear": 1, "mlp": 2}
 
 STATUS_NAMES = {
@@ -139,6 +141,19 @@ SIGNATURES = {
     "bgnn_dist_set_row_blocks": [_P, _U32],
     "bgnn_dist_allreduce_max": [_P, ctypes.POINTER(_D), _U32],
     "bgnn_dist_synchronize": [_P],
+    "bgnn_rms_norm": [_P, _I, _P, _U64, _I, _P, _U64, _I, _P, _U64, _U32, _D, _P, _I, _P, _P],
+    "bgnn_rms_norm_backward": [_P, _I, _P, _U64, _I, _P, _U64, _P, _U64, _I, _P, _U64, _U32, _D,
+                               _P, _P],
+    "bgnn_linear_fused": [_P, _I, _P, _U64, _P, _P, _U64, _P, _U64, _U32, _U32, _I, _P, _I, _D,
+                          _I, _P, _U64, _I, _P, _U64],
+    "bgnn_linear_fused_backward": [_P, _I, _P, _U64, _P, _U64, _P, _U64, _U64, _U32, _U32, _I, _P,
+                                   _I, _D, _P, _P, _P],
+    "bgnn_gated_linear": [_P, _I, _P, _U64, _P, _P, _U64, _P, _P, _U64, _P, _U64, _U32, _U32, _I,
+                          _P, _P, _I, _D, _I, _P, _U64],
+    "bgnn_gated_linear_backward": [_P, _I, _P, _U64, _P, _U64, _P, _U64, _P, _U64, _U64, _U32,
+                                   _U32, _I, _P, _P, _I, _D, _P, _P, _P, _P, _P],
+    "bgnn_log_probs": [_P, _I, _P, _U64, _U32, _U32, _P, _U64, _P, _U32, _P, _P, _P, _P, _P],
+    "bgnn_log_probs_backward": [_P, _I, _P, _U64, _U32, _U32, _P, _U64, _P, _P, _P, _P, _P, _P],
 }
 _RESTYPE = {"bgnn_last_error": ctypes.c_char_p, "bgnn_ctx_launch_count": ctypes.c_uint64}
 

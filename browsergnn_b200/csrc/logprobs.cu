@@ -1,0 +1,533 @@
+// Log probabilities of each row's given choice, with the entropy, the
+// log-sum-exp and the top alternatives; and their gradient.
+//
+// Over the choices that are left in a row (not masked, logit above -inf):
+//   lse = m + log S,  S = sum_j exp(x_j - m),  m = max_j x_j
+//   logp_t = (x_t - m) - log S
+//   H = -sum_j p_j log p_j = log S - (1/S) sum_j (x_j - m) exp(x_j - m)
+// and, for the gradients g_l of logp_t and g_h of H,
+//   dx_j = p_j (-g_l - g_h (log p_j + H)) + g_l [j = t],   p_j = exp(x_j - lse).
+//
+// One pass: every thread keeps a running (m, S, W = sum (x - m) exp(x - m))
+// in f32 and rescales it when its maximum moves (W' = e^(m-m') (W + (m-m') S));
+// pairs merge the same way.  The top list lives sorted in a warp's lanes
+// (lane i: the i-th best); an element enters when it beats the last of the
+// list, so after the first few hundred elements the test is one comparison a
+// vector.  A long row is split over blocks and joined by k_logp_join; short
+// rows take a warp each.  Memory bound: the logits (and masks) are read once.
+#include "lowp.cuh"
+
+namespace {
+
+constexpr uint32_t NO_CHOICE = 0xffffffffu;
+constexpr int TOP_MAX = 32;
+constexpr int LP_WARPS = 8;  // of a block in the split kernel
+
+struct LogpArgs {
+  const void* x;
+  uint64_t ld;
+  uint32_t rows, cols;
+  const uint8_t* mask;  // may be NULL
+  uint64_t ld_mask;     // 0: one mask for all rows
+  const uint32_t* targets;
+  int top;
+  uint32_t splits, seg;  // a row is cut into `splits` segments of `seg` elements
+  float* logp;
+  float* entropy;
+  float* lse;
+  uint32_t* top_ids;
+  float* top_logp;
+  float4* part;       // [rows, splits] (m, S, W, -)
+  float* part_v;      // [rows, splits, top]
+  uint32_t* part_id;  // [rows, splits, top]
+  int* err;
+};
+
+struct Stat {
+  float m, s, w;
+};
+
+__device__ __forceinline__ Stat stat_merge(Stat a, Stat b) {
+  const float m = fmaxf(a.m, b.m);
+  const float ms = m == -INFINITY ? 0.0f : m;
+  // the side with nothing in it contributes S = W = 0 whatever its m
+  const float da = a.m == -INFINITY ? 0.0f : a.m - ms, db = b.m == -INFINITY ? 0.0f : b.m - ms;
+  const float ea = __expf(da), eb = __expf(db);
+  const float sa = a.s * ea, sb = b.s * eb;
+  Stat r;
+  r.m = m;
+  r.s = sa + sb;
+  // da * sa only while sa is not 0: da may be as low as -inf (a row of the
+  // type's lowest value beside an ordinary one)
+  r.w = a.w * ea + b.w * eb + (sa != 0.0f ? da * sa : 0.0f) + (sb != 0.0f ? db * sb : 0.0f);
+  return r;
+}
+
+__device__ __forceinline__ Stat warp_stat(Stat t) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Stat u;
+    u.m = __shfl_xor_sync(0xffffffffu, t.m, o);
+    u.s = __shfl_xor_sync(0xffffffffu, t.s, o);
+    u.w = __shfl_xor_sync(0xffffffffu, t.w, o);
+    t = stat_merge(t, u);
+  }
+  return t;
+}
+
+// a before b in the list: greater value, then lower index
+__device__ __forceinline__ bool before(float av, uint32_t ai, float bv, uint32_t bi) {
+  return av > bv || (av == bv && ai < bi);
+}
+
+// a warp's sorted list of the best `top` elements, lane i holding the i-th
+struct TopList {
+  float v = -INFINITY;
+  uint32_t id = NO_CHOICE;
+  float last_v = -INFINITY;  // the last that is still in the list
+  uint32_t last_id = NO_CHOICE;
+
+  // offers one element a lane; all lanes call
+  __device__ __forceinline__ void offer(float cv, uint32_t ci, int top, int lane) {
+    if (cv == -INFINITY) ci = NO_CHOICE;  // not an alternative
+    uint32_t in = __ballot_sync(0xffffffffu, before(cv, ci, last_v, last_id));
+    while (in) {
+      const int src = __ffs((int)in) - 1;
+      const float nv = __shfl_sync(0xffffffffu, cv, src);
+      const uint32_t ni = __shfl_sync(0xffffffffu, ci, src);
+      const int pos = __popc(__ballot_sync(0xffffffffu, before(v, id, nv, ni)));
+      const float uv = __shfl_up_sync(0xffffffffu, v, 1);
+      const uint32_t ui = __shfl_up_sync(0xffffffffu, id, 1);
+      if (lane > pos) v = uv, id = ui;
+      if (lane == pos) v = nv, id = ni;
+      last_v = __shfl_sync(0xffffffffu, v, top - 1);
+      last_id = __shfl_sync(0xffffffffu, id, top - 1);
+      in &= in - 1;
+      in &= __ballot_sync(0xffffffffu, before(cv, ci, last_v, last_id));
+    }
+  }
+};
+
+// the eight elements [e, e + 8) of a row, -inf outside [lo, hi) and where masked
+template <int DT>
+__device__ __forceinline__ void load_left(const elt_t<DT>* xr, const uint8_t* mr, bool mask_vec,
+                                          int64_t e, int64_t lo, int64_t hi, float (&v)[8]) {
+  if (e >= lo && e + 8 <= hi) {
+    load8<DT>(xr + e, v);
+    if (mr) {
+      if (mask_vec) {
+        const uint2 mm = *reinterpret_cast<const uint2*>(mr + e);
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          if (((j < 4 ? mm.x >> (8 * j) : mm.y >> (8 * (j - 4))) & 0xffu) != 0) v[j] = -INFINITY;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          if (mr[e + j]) v[j] = -INFINITY;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int64_t i = e + j;
+      v[j] = (i >= lo && i < hi && !(mr && mr[i])) ? Elt<DT>::get(xr[i]) : -INFINITY;
+    }
+  }
+}
+
+// elements before the row's first that share its 8-element vector
+template <int DT>
+__device__ __forceinline__ int row_lead(const elt_t<DT>* xr) {
+  return (int)(((uintptr_t)xr / sizeof(elt_t<DT>)) & 7u);
+}
+
+__device__ __forceinline__ void stat_add(Stat& t, const float (&v)[8]) {
+  float cm = v[0];
+#pragma unroll
+  for (int j = 1; j < 8; j++) cm = fmaxf(cm, v[j]);
+  if (cm > t.m) {
+    const float d = t.m == -INFINITY ? 0.0f : t.m - cm;
+    const float e = __expf(d);
+    t.s *= e;
+    t.w = t.w * e + (t.s != 0.0f ? d * t.s : 0.0f);
+    t.m = cm;
+  }
+  const float m = t.m == -INFINITY ? 0.0f : t.m;
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const float d = v[j] - m;
+    const float e = __expf(d);
+    t.s += e;
+    t.w += d == -INFINITY ? 0.0f : d * e;
+  }
+}
+
+// one row's figures from its statistics and list; one warp
+template <int DT>
+__device__ __forceinline__ void finish_row(const LogpArgs& a, uint64_t row, Stat t,
+                                           const TopList& best, int lane) {
+  const bool empty = t.m == -INFINITY && t.s == 0.0f;
+  // a +inf logit leaves no finite difference: all figures NaN, as for a NaN
+  // logit.  x - m first: m + log S alone drops log S beside a large m.
+  const float ls = logf(t.s);
+  if (lane == 0) {
+    if (a.lse) a.lse[row] = empty ? -INFINITY : t.m + ls;
+    if (a.entropy) a.entropy[row] = empty ? 0.0f : fmaf(-t.w, __fdiv_rn(1.0f, t.s), ls);
+    if (a.logp) {
+      const uint32_t c = a.targets[row];
+      float lp = 0.0f;  // no choice given
+      if (c != NO_CHOICE) {
+        if (c >= a.cols) {
+          dev_raise(a.err, DEVERR_INDEX, c, 60);
+          lp = __int_as_float(0x7fc00000);
+        } else {
+          const bool out = a.mask && a.mask[row * a.ld_mask + c];
+          const float x = Elt<DT>::get(static_cast<const elt_t<DT>*>(a.x)[row * a.ld + c]);
+          lp = (empty || out) ? -INFINITY : (x - t.m) - ls;
+        }
+      }
+      a.logp[row] = lp;
+    }
+  }
+  if (lane < a.top) {
+    const bool some = best.v > -INFINITY;
+    a.top_ids[row * a.top + lane] = some ? best.id : NO_CHOICE;
+    a.top_logp[row * a.top + lane] = some ? (best.v - t.m) - ls : -INFINITY;
+  }
+}
+
+// rows of one segment: block = (row, segment); its warps interleave vectors
+template <int DT>
+__global__ void __launch_bounds__(LP_WARPS * 32) k_logp(const LogpArgs a) {
+  __shared__ float sm_m[LP_WARPS], sm_s[LP_WARPS], sm_w[LP_WARPS];
+  __shared__ float sm_v[LP_WARPS][TOP_MAX];
+  __shared__ uint32_t sm_id[LP_WARPS][TOP_MAX];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint64_t row = blockIdx.x / a.splits;
+  const uint32_t split = blockIdx.x % a.splits;
+  const elt_t<DT>* xr = static_cast<const elt_t<DT>*>(a.x) + row * a.ld;
+  const uint8_t* mr = a.mask ? a.mask + row * a.ld_mask : nullptr;
+  const int64_t lead = row_lead<DT>(xr);
+  const bool mask_vec = mr && (((uintptr_t)mr - (uintptr_t)lead) & 7u) == 0;
+  // segments are cut at whole vectors: [lo, hi) in elements of the row
+  const int64_t first = (int64_t)split * a.seg - lead;
+  const int64_t lo = first > 0 ? first : 0;
+  const int64_t end = first + a.seg;
+  const int64_t hi = end < (int64_t)a.cols ? end : (int64_t)a.cols;
+  Stat t = {-INFINITY, 0.0f, 0.0f};
+  TopList best;
+  for (int64_t b = first + warp * 256; b < hi; b += LP_WARPS * 256) {
+    const int64_t e = b + lane * 8;
+    float v[8];
+    load_left<DT>(xr, mr, mask_vec, e, lo, hi, v);
+    stat_add(t, v);
+    if (a.top) {
+      float cm = v[0];
+#pragma unroll
+      for (int j = 1; j < 8; j++) cm = fmaxf(cm, v[j]);
+      // strictly above: a warp sees its elements in ascending order, so an
+      // equal one comes after the one that is listed
+      if (__any_sync(0xffffffffu, cm > best.last_v)) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) best.offer(v[j], (uint32_t)(e + j), a.top, lane);
+      }
+    }
+  }
+  t = warp_stat(t);
+  if (lane == 0) sm_m[warp] = t.m, sm_s[warp] = t.s, sm_w[warp] = t.w;
+  sm_v[warp][lane] = best.v;
+  sm_id[warp][lane] = best.id;
+  __syncthreads();
+  if (warp != 0) return;
+  Stat u = {-INFINITY, 0.0f, 0.0f};
+  if (lane < LP_WARPS) u = {sm_m[lane], sm_s[lane], sm_w[lane]};
+  u = warp_stat(u);
+  if (a.top)
+    for (int w = 1; w < LP_WARPS; w++)
+      best.offer(lane < a.top ? sm_v[w][lane] : -INFINITY, lane < a.top ? sm_id[w][lane] : NO_CHOICE,
+                 a.top, lane);
+  if (a.splits == 1) {
+    finish_row<DT>(a, row, u, best, lane);
+  } else {
+    const uint64_t p = row * a.splits + split;
+    if (lane == 0) a.part[p] = make_float4(u.m, u.s, u.w, 0.0f);
+    if (lane < a.top) {
+      a.part_v[p * a.top + lane] = best.v;
+      a.part_id[p * a.top + lane] = best.id;
+    }
+  }
+}
+
+// joins a row's segments: one block a row
+template <int DT>
+__global__ void __launch_bounds__(LP_WARPS * 32) k_logp_join(const LogpArgs a) {
+  __shared__ float sm_m[LP_WARPS], sm_s[LP_WARPS], sm_w[LP_WARPS];
+  __shared__ float sm_v[LP_WARPS][TOP_MAX];
+  __shared__ uint32_t sm_id[LP_WARPS][TOP_MAX];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint64_t row = blockIdx.x;
+  Stat t = {-INFINITY, 0.0f, 0.0f};
+  for (uint32_t s = threadIdx.x; s < a.splits; s += LP_WARPS * 32) {
+    const float4 p = a.part[row * a.splits + s];
+    t = stat_merge(t, {p.x, p.y, p.z});
+  }
+  t = warp_stat(t);
+  TopList best;
+  if (a.top) {
+    const uint32_t n = a.splits * (uint32_t)a.top;
+    const uint64_t at = row * n;
+    for (uint32_t b = warp * 32; b < n; b += LP_WARPS * 32) {
+      const bool on = b + lane < n;
+      best.offer(on ? a.part_v[at + b + lane] : -INFINITY, on ? a.part_id[at + b + lane] : NO_CHOICE,
+                 a.top, lane);
+    }
+  }
+  if (lane == 0) sm_m[warp] = t.m, sm_s[warp] = t.s, sm_w[warp] = t.w;
+  sm_v[warp][lane] = best.v;
+  sm_id[warp][lane] = best.id;
+  __syncthreads();
+  if (warp != 0) return;
+  Stat u = {-INFINITY, 0.0f, 0.0f};
+  if (lane < LP_WARPS) u = {sm_m[lane], sm_s[lane], sm_w[lane]};
+  u = warp_stat(u);
+  if (a.top)
+    for (int w = 1; w < LP_WARPS; w++)
+      best.offer(lane < a.top ? sm_v[w][lane] : -INFINITY, lane < a.top ? sm_id[w][lane] : NO_CHOICE,
+                 a.top, lane);
+  finish_row<DT>(a, row, u, best, lane);
+}
+
+// short rows: a warp a row
+template <int DT>
+__global__ void __launch_bounds__(LP_WARPS * 32) k_logp_short(const LogpArgs a) {
+  const int lane = threadIdx.x & 31;
+  const uint64_t step = (uint64_t)gridDim.x * LP_WARPS;
+  for (uint64_t row = (uint64_t)blockIdx.x * LP_WARPS + (threadIdx.x >> 5); row < a.rows;
+       row += step) {
+    const elt_t<DT>* xr = static_cast<const elt_t<DT>*>(a.x) + row * a.ld;
+    const uint8_t* mr = a.mask ? a.mask + row * a.ld_mask : nullptr;
+    const int64_t lead = row_lead<DT>(xr), hi = a.cols;
+    const bool mask_vec = mr && (((uintptr_t)mr - (uintptr_t)lead) & 7u) == 0;
+    Stat t = {-INFINITY, 0.0f, 0.0f};
+    TopList best;
+    for (int64_t b = -lead; b < hi; b += 256) {
+      const int64_t e = b + lane * 8;
+      float v[8];
+      load_left<DT>(xr, mr, mask_vec, e, 0, hi, v);
+      stat_add(t, v);
+      if (a.top) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) best.offer(v[j], (uint32_t)(e + j), a.top, lane);
+      }
+    }
+    finish_row<DT>(a, row, warp_stat(t), best, lane);
+  }
+}
+
+struct LogpBwdArgs {
+  const void* x;
+  uint64_t ld;
+  uint32_t rows, cols;
+  const uint8_t* mask;
+  uint64_t ld_mask;
+  const uint32_t* targets;
+  const float* lse;
+  const float* entropy;
+  const float* g_logp;
+  const float* g_ent;  // either may be NULL
+  void* dx;            // [rows, cols]
+  uint32_t splits, seg;
+  int* err;
+};
+
+// From |lse| = 128 on, its last bit is worth 2^-17 and more of a probability:
+// such a row's m and log S are summed again by every block that works on it.
+constexpr float LSE_EXACT = 128.0f;
+
+template <int DT>
+__global__ void __launch_bounds__(256) k_logp_bwd(const LogpBwdArgs a) {
+  __shared__ float sm_m[8], sm_s[8];
+  const uint64_t units = (uint64_t)a.rows * a.splits;
+  for (uint64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const uint64_t row = u / a.splits;
+    const uint32_t split = (uint32_t)(u % a.splits);
+    const elt_t<DT>* xr = static_cast<const elt_t<DT>*>(a.x) + row * a.ld;
+    elt_t<DT>* dr = static_cast<elt_t<DT>*>(a.dx) + row * a.cols;
+    const uint8_t* mr = a.mask ? a.mask + row * a.ld_mask : nullptr;
+    const int64_t lead = row_lead<DT>(xr);
+    const bool mask_vec = mr && (((uintptr_t)mr - (uintptr_t)lead) & 7u) == 0;
+    const bool out_vec = (((uintptr_t)dr - (uintptr_t)lead * sizeof(elt_t<DT>)) & 15u) == 0;
+    const int64_t first = (int64_t)split * a.seg - lead;
+    const int64_t lo = first > 0 ? first : 0;
+    const int64_t end = first + a.seg;
+    const int64_t hi = end < (int64_t)a.cols ? end : (int64_t)a.cols;
+    const uint32_t c = a.targets[row];
+    const float lse = a.lse[row];
+    const float gl = a.g_logp && c != NO_CHOICE ? a.g_logp[row] : 0.0f;
+    const float gh = a.g_ent ? a.g_ent[row] : 0.0f;
+    const float h = a.g_ent ? a.entropy[row] : 0.0f;
+    if (c != NO_CHOICE && c >= a.cols && split == 0 && threadIdx.x == 0)
+      dev_raise(a.err, DEVERR_INDEX, c, 61);
+    const float k0 = fmaf(-gh, h, -gl);
+    float m = 0.0f, ls = lse;  // log p = (x - m) - ls
+    if (fabsf(lse) >= LSE_EXACT && fabsf(lse) < INFINITY) {
+      Stat t = {-INFINITY, 0.0f, 0.0f};
+      for (int64_t e = (int64_t)threadIdx.x * 8 - lead; e < (int64_t)a.cols; e += 256 * 8) {
+        float v[8];
+        load_left<DT>(xr, mr, mask_vec, e, 0, a.cols, v);
+        stat_add(t, v);
+      }
+      t = warp_stat(t);
+      __syncthreads();  // the last unit's reads
+      if ((threadIdx.x & 31) == 0) sm_m[threadIdx.x >> 5] = t.m, sm_s[threadIdx.x >> 5] = t.s;
+      __syncthreads();
+      t = {sm_m[0], sm_s[0], 0.0f};
+      for (int i = 1; i < 8; i++) t = stat_merge(t, {sm_m[i], sm_s[i], 0.0f});
+      m = t.m;
+      ls = logf(t.s);
+    }
+    for (int64_t e = first + (int64_t)threadIdx.x * 8; e < hi; e += 256 * 8) {
+      float v[8];
+      load_left<DT>(xr, mr, mask_vec, e, lo, hi, v);
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        // what is not left, and all of an empty row, has p = 0 and no gradient
+        const float lp = (v[j] - m) - ls;
+        float d = v[j] == -INFINITY ? 0.0f : __expf(lp) * fmaf(-gh, lp, k0);
+        if (e + j == (int64_t)c && v[j] != -INFINITY) d += gl;
+        v[j] = d;
+      }
+      if (out_vec && e >= lo && e + 8 <= hi) {
+        store8<DT>(dr + e, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          if (e + j >= lo && e + j < hi) dr[e + j] = Elt<DT>::put(v[j]);
+      }
+    }
+  }
+}
+
+// Segments of a row so that rows * segments fill the GPU's resident blocks;
+// a segment keeps at least `least` elements and is whole vectors.
+void cut_rows(const bgnn_ctx* ctx, uint32_t rows, uint32_t cols, uint32_t blocks_per_sm,
+              uint32_t least, uint32_t* splits, uint32_t* seg) {
+  const uint64_t want = (uint64_t)ctx->num_sms * blocks_per_sm;
+  uint64_t s = rows >= want ? 1 : want / rows;
+  const uint64_t most = ((uint64_t)cols + least - 1) / least;
+  if (s > most) s = most;
+  if (s < 1) s = 1;
+  // + 7: the first vector may start before the row
+  uint64_t n = (((uint64_t)cols + 7 + s - 1) / s + 2047) / 2048 * 2048;
+  if (s == 1) n = ((uint64_t)cols + 7 + 7) / 8 * 8;
+  *seg = (uint32_t)n;
+  *splits = (uint32_t)(((uint64_t)cols + 7 + n - 1) / n);
+}
+
+constexpr uint32_t LP_SHORT = 1024;  // columns up to which a row takes a warp
+
+template <int DT>
+int run_logp(bgnn_ctx* ctx, LogpArgs a) {
+  if (a.cols <= LP_SHORT) {
+    const uint64_t want = ((uint64_t)a.rows + LP_WARPS - 1) / LP_WARPS;
+    const uint64_t cap = (uint64_t)ctx->num_sms * 8;
+    k_logp_short<DT><<<(unsigned)(want < cap ? want : cap), LP_WARPS * 32, 0, ctx->stream>>>(a);
+    BGNN_LAUNCHED(ctx);
+    return BGNN_OK;
+  }
+  cut_rows(ctx, a.rows, a.cols, 4, 8192, &a.splits, &a.seg);
+  DevTmp ws;
+  const uint64_t parts = (uint64_t)a.rows * a.splits;
+  if (a.splits > 1) {
+    BGNN_TRY(bgnn_tmp_alloc(ctx, ws, parts * (sizeof(float4) + 8 * (uint64_t)a.top)));
+    a.part = ws.as<float4>();
+    a.part_v = reinterpret_cast<float*>(a.part + parts);
+    a.part_id = reinterpret_cast<uint32_t*>(a.part_v + parts * a.top);
+  }
+  k_logp<DT><<<(unsigned)parts, LP_WARPS * 32, 0, ctx->stream>>>(a);
+  BGNN_LAUNCHED(ctx);
+  if (a.splits > 1) {
+    k_logp_join<DT><<<a.rows, LP_WARPS * 32, 0, ctx->stream>>>(a);
+    BGNN_LAUNCHED(ctx);
+  }
+  return BGNN_OK;
+}
+
+template <int DT>
+int run_logp_bwd(bgnn_ctx* ctx, LogpBwdArgs a) {
+  cut_rows(ctx, a.rows, a.cols, 8, 2048, &a.splits, &a.seg);
+  const uint64_t units = (uint64_t)a.rows * a.splits, cap = (uint64_t)ctx->num_sms * 64;
+  k_logp_bwd<DT><<<(unsigned)(units < cap ? units : cap), 256, 0, ctx->stream>>>(a);
+  BGNN_LAUNCHED(ctx);
+  return BGNN_OK;
+}
+
+}  // namespace
+
+extern "C" int bgnn_log_probs(bgnn_ctx* ctx, int type, const void* logits, uint64_t ld,
+                              uint32_t rows, uint32_t cols, const uint8_t* mask, uint64_t ld_mask,
+                              const uint32_t* targets, uint32_t top_k, float* logp, float* entropy,
+                              float* lse, uint32_t* top_ids, float* top_logp) {
+  BGNN_ON_DEVICE(ctx);
+  BGNN_REQUIRE(ctx, dtype_float(type), "log_probs: unknown element type %d", type);
+  BGNN_REQUIRE(ctx, top_k <= TOP_MAX, "log_probs: top_k %u above %d", top_k, TOP_MAX);
+  if (rows == 0) return BGNN_OK;
+  BGNN_REQUIRE(ctx, logits || cols == 0, "log_probs: NULL logits");
+  BGNN_REQUIRE(ctx, ld >= cols && (!mask || ld_mask == 0 || ld_mask >= cols),
+               "log_probs: row stride below the row length");
+  BGNN_REQUIRE(ctx, !logp || targets, "log_probs: logp needs targets");
+  BGNN_REQUIRE(ctx, top_k == 0 || (top_ids && top_logp), "log_probs: NULL top list");
+  LogpArgs a = {};
+  a.x = logits;
+  a.ld = ld;
+  a.rows = rows;
+  a.cols = cols;
+  a.mask = cols ? mask : nullptr;
+  a.ld_mask = ld_mask;
+  a.targets = targets;
+  a.top = (int)top_k;
+  a.logp = logp;
+  a.entropy = entropy;
+  a.lse = lse;
+  a.top_ids = top_ids;
+  a.top_logp = top_logp;
+  a.err = ctx->d_err;
+  switch (type) {
+    case BGNN_F32: return run_logp<BGNN_F32>(ctx, a);
+    case BGNN_BF16: return run_logp<BGNN_BF16>(ctx, a);
+    default: return run_logp<BGNN_F16>(ctx, a);
+  }
+}
+
+extern "C" int bgnn_log_probs_backward(bgnn_ctx* ctx, int type, const void* logits, uint64_t ld,
+                                       uint32_t rows, uint32_t cols, const uint8_t* mask,
+                                       uint64_t ld_mask, const uint32_t* targets, const float* lse,
+                                       const float* entropy, const float* grad_logp,
+                                       const float* grad_entropy, void* grad_logits) {
+  BGNN_ON_DEVICE(ctx);
+  BGNN_REQUIRE(ctx, dtype_float(type), "log_probs_backward: unknown element type %d", type);
+  if (rows == 0 || cols == 0) return BGNN_OK;
+  BGNN_REQUIRE(ctx, logits && targets && lse && grad_logits, "log_probs_backward: NULL argument");
+  BGNN_REQUIRE(ctx, !grad_entropy || entropy, "log_probs_backward: grad_entropy needs the entropy");
+  BGNN_REQUIRE(ctx, ld >= cols && (!mask || ld_mask == 0 || ld_mask >= cols),
+               "log_probs_backward: row stride below the row length");
+  LogpBwdArgs a = {};
+  a.x = logits;
+  a.ld = ld;
+  a.rows = rows;
+  a.cols = cols;
+  a.mask = mask;
+  a.ld_mask = ld_mask;
+  a.targets = targets;
+  a.lse = lse;
+  a.entropy = entropy;
+  a.g_logp = grad_logp;
+  a.g_ent = grad_entropy;
+  a.dx = grad_logits;
+  a.err = ctx->d_err;
+  switch (type) {
+    case BGNN_F32: return run_logp_bwd<BGNN_F32>(ctx, a);
+    case BGNN_BF16: return run_logp_bwd<BGNN_BF16>(ctx, a);
+    default: return run_logp_bwd<BGNN_F16>(ctx, a);
+  }
+}

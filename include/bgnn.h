@@ -99,6 +99,15 @@ typedef enum bgnn_link_mode {
   BGNN_LINK_MLP = 2       /* sigmoid(Linear(ReLU(Linear([s,t,s*t]))))   */
 } bgnn_link_mode;
 
+/* element types of the mixed-precision operators (the block operators and
+ * the choice head below); everything else is f32 */
+typedef enum bgnn_dtype {
+  BGNN_F32 = 0,
+  BGNN_BF16 = 1,
+  BGNN_F16 = 2,
+  BGNN_E4M3 = 3 /* 8 bits, with f32 scales */
+} bgnn_dtype;
+
 typedef struct bgnn_ctx bgnn_ctx;
 typedef struct bgnn_graph bgnn_graph;
 
@@ -539,6 +548,118 @@ BGNN_API int bgnn_link_scores(bgnn_ctx* ctx, const float* emb, uint32_t num_node
                               const uint32_t* src, const uint32_t* tgt, uint64_t num_pairs,
                               int mode, const float* w_bilinear, const float* w1, const float* b1,
                               const float* w2, const float* b2, double* out);
+
+/* ---- block operators: norm, gated and plain products, mixed precision ------
+ * No counterpart in the reference, whose dense layers are f32: what a model
+ * puts between its message-passing layers and at its end, with 16- and 8-bit
+ * operands.  Types are bgnn_dtype; device pointers, asynchronous on the
+ * context's stream; row strides (ld_*) count elements and are at least the
+ * row length; outputs without a stride are contiguous; inputs and outputs do
+ * not overlap unless said.  Sums, statistics and epilogues are f32 and every
+ * output is rounded once. */
+
+/* Root-mean-square norm with the residual's addition:
+ *   t = x + residual, rounded to the residual's type -> total [rows, cols]
+ *       (t = x and total unused when residual is NULL; total may be the
+ *       residual's own buffer when ld_res == cols)
+ *   y = t * (mean(t^2) + eps)^(-1/2) * weight
+ *   out = y, or for BGNN_E4M3 y / scale[row] with scale = max|y| / 448 (1 for
+ *       an all-zero row; e4m3 rounds to nearest even).
+ * x f32, bf16 or f16; the residual has x's type or f32; weight [cols] any of
+ * the three; out f32, bf16, f16 or e4m3 (scale [rows], else NULL).  A row that
+ * holds a NaN or an infinity gives NaN in what it touches, and a NaN scale or
+ * an infinite one. */
+BGNN_API int bgnn_rms_norm(bgnn_ctx* ctx, int x_type, const void* x, uint64_t ld_x, int res_type,
+                           const void* residual, uint64_t ld_res, int w_type, const void* weight,
+                           uint64_t rows, uint32_t cols, double eps, void* total, int out_type,
+                           void* out, float* scale);
+/* Its gradients from the forward's `total` (or x): grad_x [rows, cols] in
+ * total's type is the gradient of x and of the residual alike, grad_total
+ * (may be NULL, total's type) being the gradient that reaches total along the
+ * residual stream; grad_weight [cols] in weight's type (may be NULL).  grad
+ * has total's type, or any when total is f32. */
+BGNN_API int bgnn_rms_norm_backward(bgnn_ctx* ctx, int grad_type, const void* grad,
+                                    uint64_t ld_grad, int total_type, const void* total,
+                                    uint64_t ld_total, const void* grad_total,
+                                    uint64_t ld_grad_total, int w_type, const void* weight,
+                                    uint64_t rows, uint32_t cols, double eps, void* grad_x,
+                                    void* grad_weight);
+
+/* out [m, n] = act(x w^T + bias) + residual on the tensor cores, w [n, k] as
+ * in bgnn_dense.  type: of x and w, bf16 or f16, or e4m3 with one scale a row
+ * (x_scale [m], w_scale [n]; NULL otherwise).  bias [n], residual and out are
+ * f32, bf16 or f16; bias and residual may be NULL.  act: bgnn_act, evaluated
+ * in f32.  An operand whose rows do not start on 16 bytes is copied to rows
+ * that do.  out may be the residual's own buffer. */
+BGNN_API int bgnn_linear_fused(bgnn_ctx* ctx, int type, const void* x, uint64_t ld_x,
+                               const float* x_scale, const void* w, uint64_t ld_w,
+                               const float* w_scale, uint64_t m, uint32_t k, uint32_t n,
+                               int bias_type, const void* bias, int act, double act_param,
+                               int res_type, const void* residual, uint64_t ld_res, int out_type,
+                               void* out, uint64_t ld_out);
+/* Its gradients for an upstream gradient grad [m, n] (type bf16 or f16, as x
+ * and w): with z = x w^T + bias computed once more and dz = grad act'(z)
+ * rounded to `type`, grad_x = dz w, grad_w = dz^T x (both in `type`),
+ * grad_bias = column sums of dz (bias_type).  The residual's gradient is grad.
+ * Any of the three may be NULL.  Sums run in a fixed order. */
+BGNN_API int bgnn_linear_fused_backward(bgnn_ctx* ctx, int type, const void* grad,
+                                        uint64_t ld_grad, const void* x, uint64_t ld_x,
+                                        const void* w, uint64_t ld_w, uint64_t m, uint32_t k,
+                                        uint32_t n, int bias_type, const void* bias, int act,
+                                        double act_param, void* grad_x, void* grad_w,
+                                        void* grad_bias);
+/* out [m, n] = act(x w_gate^T + bias_gate) * (x w_up^T + bias_up), both
+ * products, the activation and the product in one kernel; types and scales as
+ * bgnn_linear_fused.  Either bias may be NULL. */
+BGNN_API int bgnn_gated_linear(bgnn_ctx* ctx, int type, const void* x, uint64_t ld_x,
+                               const float* x_scale, const void* w_gate, uint64_t ld_gate,
+                               const float* gate_scale, const void* w_up, uint64_t ld_up,
+                               const float* up_scale, uint64_t m, uint32_t k, uint32_t n,
+                               int bias_type, const void* bias_gate, const void* bias_up, int act,
+                               double act_param, int out_type, void* out, uint64_t ld_out);
+/* Its gradients: both products once more, dg = grad u act'(zg) and
+ * du = grad act(zg) rounded to `type`, grad_x = dg w_gate + du w_up,
+ * grad_w_gate = dg^T x, grad_w_up = du^T x, bias gradients the column sums.
+ * Any output may be NULL (the two weight gradients together). */
+BGNN_API int bgnn_gated_linear_backward(bgnn_ctx* ctx, int type, const void* grad,
+                                        uint64_t ld_grad, const void* x, uint64_t ld_x,
+                                        const void* w_gate, uint64_t ld_gate, const void* w_up,
+                                        uint64_t ld_up, uint64_t m, uint32_t k, uint32_t n,
+                                        int bias_type, const void* bias_gate, const void* bias_up,
+                                        int act, double act_param, void* grad_x,
+                                        void* grad_w_gate, void* grad_w_up, void* grad_bias_gate,
+                                        void* grad_bias_up);
+
+/* ---- choice head ------------------------------------------------------------
+ * Log probabilities of each row's given choice (a class, or a node of
+ * LearningPathRecommender.ts:173-225's softmax over nodes).  logits
+ * [rows, cols] f32, bf16 or f16; mask (may be NULL) takes out choice c of row
+ * r where mask[r * ld_mask + c] != 0, ld_mask == 0 being one mask for all
+ * rows.  A choice is left when it is not masked and its logit is above -inf.
+ *   lse [rows]      log sum_left exp(x)             (-inf when nothing is left)
+ *   logp [rows]     x[target] - lse; -inf when the target is not left; 0 when
+ *                   the target is 0xffffffff (no choice given)
+ *   entropy [rows]  -sum p log p                    (0 when nothing is left)
+ *   top_ids, top_logp [rows, top_k]  the top_k most probable choices left,
+ *                   equal logits in ascending index; 0xffffffff / -inf beyond
+ *                   the last.  top_k <= 32.
+ * logp, entropy and lse may be NULL.  A row with a NaN or +inf among what is
+ * left has NaN figures; a NaN is never an alternative.  A target >= cols is
+ * reported as BGNN_ERR_OUT_OF_RANGE at the next synchronising call (its logp
+ * is NaN). */
+BGNN_API int bgnn_log_probs(bgnn_ctx* ctx, int type, const void* logits, uint64_t ld,
+                            uint32_t rows, uint32_t cols, const uint8_t* mask, uint64_t ld_mask,
+                            const uint32_t* targets, uint32_t top_k, float* logp, float* entropy,
+                            float* lse, uint32_t* top_ids, float* top_logp);
+/* grad_logits [rows, cols] (the logits' type) for the gradients grad_logp and
+ * grad_entropy [rows] (either may be NULL) of the forward's outputs, from its
+ * lse and entropy: p (-g_l - g_h (log p + H)) + g_l [c = target], 0 for a
+ * choice that is not left. */
+BGNN_API int bgnn_log_probs_backward(bgnn_ctx* ctx, int type, const void* logits, uint64_t ld,
+                                     uint32_t rows, uint32_t cols, const uint8_t* mask,
+                                     uint64_t ld_mask, const uint32_t* targets, const float* lse,
+                                     const float* entropy, const float* grad_logp,
+                                     const float* grad_entropy, void* grad_logits);
 
 #ifdef __cplusplus
 }
