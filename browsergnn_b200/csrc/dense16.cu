@@ -40,6 +40,7 @@
 #include <cudaTypedefs.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "lowp.cuh"
 
@@ -50,19 +51,26 @@ constexpr int EPI_WARPS = 8;
 constexpr int THREADS = (EPI_WARPS + 2) * 32;
 constexpr int MAX_STAGES = 8;
 constexpr int A_BYTES = BM * 128;
-constexpr int TURN_BYTES = 32 * 32 * 4;  // an epilogue warp's turning buffer
-constexpr int RING_BYTES = 192 * 1024;
-constexpr int SMEM_BYTES = 1024 + RING_BYTES + EPI_WARPS * TURN_BYTES + 512;
+constexpr int SLOT_BYTES = 32 * 32 * 4;     // a 32 x 32 chunk in f32
+constexpr int WARP_BYTES = 2 * SLOT_BYTES;  // an epilogue warp's chunk in and chunk out
+constexpr int RING_BYTES = 160 * 1024;
+constexpr int SMEM_BYTES = 1024 + RING_BYTES + EPI_WARPS * WARP_BYTES + 512;
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory of one SM");
 constexpr uint32_t SPIN_LIMIT = 1u << 24;     // polls before a wait gives up,
 constexpr uint64_t SPIN_NS = 2000000000ull;  // or this long
 
-enum Epi : int { EPI_LINEAR, EPI_GATED, EPI_LINEAR_BWD, EPI_GATED_BWD, EPI_PARTIAL };
+enum Epi : int { EPI_LINEAR, EPI_LINEAR_F32, EPI_GATED, EPI_LINEAR_BWD, EPI_GATED_BWD, EPI_PARTIAL };
+// k blocks whose products one accumulator takes before they are added in f32
+// registers, where the result stays f32 (EPI_LINEAR_F32)
+constexpr uint32_t PIECE = 8;
+constexpr uint32_t MAX_PER = 512;  // k blocks of a dw range
 
 // One contraction segment: A [m, k] and B [n, k] tiles of one or two tensors.
 // Where `b1` is used (gated), B's tile is rows of b0 above rows of b1.
+// in / out: the residual or upstream gradient and the outputs in 32 x 32 boxes,
+// where TMA can take them.
 struct Maps {
-  CUtensorMap a[2], b[2];
+  CUtensorMap a[2], b[2], in, out[2];
 };
 
 struct GemmArgs {
@@ -89,7 +97,8 @@ struct GemmArgs {
   int out_type;
   void* out[2];           // gated backward: dg and du; dw: one a batch
   uint64_t ld_out;
-  float* part;            // EPI_PARTIAL: [splits, batches, m, n]
+  int tma_in, tma_out;    // maps.in, maps.out are set
+  uint32_t part_rows;     // EPI_PARTIAL: rows of a partial matrix (0: dw whole, no parts)
   int* err;
 };
 
@@ -103,9 +112,6 @@ __device__ __forceinline__ void mbar_init(uint32_t a, uint32_t count) {
 __device__ __forceinline__ void mbar_expect_tx(uint32_t a, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(a), "r"(bytes)
                : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t a) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(a) : "memory");
 }
 __device__ __forceinline__ bool mbar_try(uint32_t a, uint32_t parity) {
   uint32_t ok;
@@ -142,13 +148,75 @@ __device__ __forceinline__ void mbar_drain(uint32_t a, uint32_t parity) {
   for (uint32_t i = 0; i < SPIN_LIMIT; i++)
     if (mbar_try(a, parity) || now_ns() - t0 > SPIN_NS / 4) return;
 }
+// CG: CTAs that share one product (cta_group), 1 or a pair
+template <int CG>
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y,
                                             uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
-      : "memory");
+  if constexpr (CG == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2"
+        " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// the cluster address of this CTA's shared address `a` in the CTA `rank`
+__device__ __forceinline__ uint32_t peer_addr(uint32_t a, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+  return r;
+}
+// arrives on the issuing CTA's barrier
+template <int CG>
+__device__ __forceinline__ void mbar_arrive_at(uint32_t a) {
+  if constexpr (CG == 2)
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                     peer_addr(a, 0))
+                 : "memory");
+  else
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(a) : "memory");
+}
+// all threads of the CTA, or of the pair
+template <int CG>
+__device__ __forceinline__ void pair_sync() {
+  __syncthreads();
+  if constexpr (CG == 2) {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t cols) {
+  if constexpr (CG == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot),
+                 "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot),
+                 "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_free(uint32_t t, uint32_t cols) {
+  if constexpr (CG == 2)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(t), "r"(cols)
+                 : "memory");
+  else
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(t), "r"(cols)
+                 : "memory");
 }
 // Shared-memory matrix descriptor, 128-byte swizzle, version 1.  Eight-row
 // groups (K-major: 8 rows of m or n; MN-major: 8 rows of k) are 1024 bytes
@@ -157,26 +225,61 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t a, int mn_major) {
   return (uint64_t)((a & 0x3FFFFu) >> 4) | ((uint64_t)(mn_major ? 8192 >> 4 : 1) << 16) |
          ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
+template <int CG>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                         uint32_t acc) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
+  if constexpr (CG == 2)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
 }
+template <int CG>
 __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                       uint32_t acc) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
+                                        uint32_t acc) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
 }
+// arrives on this CTA's barrier when the products issued so far are done
+template <int CG>
+__device__ __forceinline__ void mma_commit_here(uint32_t bar) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+        : "memory");
+}
+// ... and on the same barrier of the other CTA of a pair
+template <int CG>
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   bar)
-               : "memory");
+  if constexpr (CG == 2)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+  else
+    mma_commit_here<CG>(bar);
 }
 __device__ __forceinline__ void tc_fence_after() {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -184,84 +287,223 @@ __device__ __forceinline__ void tc_fence_after() {
 __device__ __forceinline__ void tc_fence_before() {
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 }
-// 32 columns of this warp's 32 lanes
+// 32 columns of this warp's 32 lanes; the values are there after tmem_wait_ld
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
-  uint32_t r[32];
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
       "%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
-        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]),
+        "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]),
+        "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]),
+        "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+        "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]),
+        "=f"(v[30]), "=f"(v[31])
       : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int j = 0; j < 32; j++) v[j] = __uint_as_float(r[j]);
+}
+// the registers pass through, so that no use of them moves before the wait
+__device__ __forceinline__ void tmem_wait_ld(float (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+      : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]),
+        "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]),
+        "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]),
+        "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]),
+        "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]),
+        "+f"(v[30]), "+f"(v[31])
+      :
+      : "memory");
 }
 
 // ---- activations, f32 ----------------------------------------------------------
-__device__ __forceinline__ float sigmoid_f(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
-constexpr float GELU_C = 0.7978845608028654f;  // sqrt(2/pi)
-__device__ __forceinline__ float gelu_arg(float z) {
-  return GELU_C * z * fmaf(0.044715f * z, z, 1.0f);
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
-__device__ __forceinline__ float act_f(float z, int act, float p) {
-  switch (act) {
-    case BGNN_ACT_RELU: return z > 0.0f ? z : 0.0f;
-    case BGNN_ACT_RELU_MAX: return z != z ? z : (z > 0.0f ? z : 0.0f);
-    case BGNN_ACT_ELU: return z > 0.0f ? z : p * expm1f(z);
-    case BGNN_ACT_LEAKY_RELU: return z > 0.0f ? z : p * z;
-    case BGNN_ACT_SIGMOID: return sigmoid_f(z);
-    case BGNN_ACT_TANH: return tanhf(z);
-    case BGNN_ACT_GELU: return z * sigmoid_f(2.0f * gelu_arg(z));  // 0.5 (1 + tanh v)
-    case BGNN_ACT_SILU: return z * sigmoid_f(z);
-    default: return z;
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float LOG2E = 1.4426950408889634f;
+// the logistic function 1 / (1 + 2^t), t = -x log2(e)
+__device__ __forceinline__ float sigmoid_t(float t) { return rcp(1.0f + ex2(t)); }
+// ... of two arguments with one reciprocal, 1/a = b/(ab): the epilogue's
+// exponentials and reciprocals share one unit of 16 lanes a clock.  t is held
+// at 63, so that ab stays finite; beyond, the value is 2^-63 instead of less,
+// which only ever enters as z * sigmoid (|z| > 43: 1e-17 of z).
+__device__ __forceinline__ float2 sigmoid_t2(float t0, float t1) {
+  const float a = 1.0f + ex2(fminf(t0, 63.0f)), b = 1.0f + ex2(fminf(t1, 63.0f));
+  const float r = rcp(a * b);
+  return make_float2(r * b, r * a);
+}
+constexpr float GELU_C = 0.7978845608028654f;  // sqrt(2/pi)
+// 0.5 (1 + tanh v) = sigmoid(2 v), v = sqrt(2/pi) (z + 0.044715 z^3), as t
+__device__ __forceinline__ float gelu_t(float z) {
+  constexpr float C = -2.0f * LOG2E * GELU_C;
+  return z * fmaf(C * 0.044715f, z * z, C);
+}
+template <int ACT>
+constexpr bool GATES = ACT == BGNN_ACT_SILU || ACT == BGNN_ACT_GELU;  // z sigmoid(..)
+template <int ACT>
+__device__ __forceinline__ float gate_t(float z) {
+  return ACT == BGNN_ACT_SILU ? -LOG2E * z : gelu_t(z);
+}
+template <int ACT>
+__device__ __forceinline__ float act_one(float z, float p) {
+  if constexpr (ACT == BGNN_ACT_RELU) return z > 0.0f ? z : 0.0f;
+  if constexpr (ACT == BGNN_ACT_RELU_MAX) return z != z ? z : (z > 0.0f ? z : 0.0f);
+  if constexpr (ACT == BGNN_ACT_ELU) return z > 0.0f ? z : p * expm1f(z);
+  if constexpr (ACT == BGNN_ACT_LEAKY_RELU) return z > 0.0f ? z : p * z;
+  if constexpr (ACT == BGNN_ACT_SIGMOID) return sigmoid_t(-LOG2E * z);
+  if constexpr (ACT == BGNN_ACT_TANH) return tanhf(z);
+  return z;
+}
+// two activations
+template <int ACT>
+__device__ __forceinline__ void act_two(float& z0, float& z1, float p) {
+  if constexpr (GATES<ACT>) {
+    const float2 s = sigmoid_t2(gate_t<ACT>(z0), gate_t<ACT>(z1));
+    z0 *= s.x;
+    z1 *= s.y;
+  } else {
+    z0 = act_one<ACT>(z0, p);
+    z1 = act_one<ACT>(z1, p);
   }
 }
-// act(z) and act'(z)
-__device__ __forceinline__ float2 act_both(float z, int act, float p) {
+// act(z) and act'(z); s: sigmoid(..) of the gates
+template <int ACT>
+__device__ __forceinline__ float2 act_grad(float z, float s, float p) {
+  if constexpr (ACT == BGNN_ACT_SILU) return make_float2(z * s, s * fmaf(z, 1.0f - s, 1.0f));
+  if constexpr (ACT == BGNN_ACT_GELU) {
+    const float dv = 2.0f * GELU_C * fmaf(3.0f * 0.044715f * z, z, 1.0f);
+    // far out s (1 - s) is 0, or z s is 2^-63 z; dv must not make a NaN of it
+    const float q = s * (1.0f - s);
+    return make_float2(z * s, q < 1e-18f ? s : fmaf(z * q, dv, s));
+  }
+  if constexpr (ACT == BGNN_ACT_RELU)
+    return z > 0.0f ? make_float2(z, 1.0f) : make_float2(0.0f, 0.0f);
+  if constexpr (ACT == BGNN_ACT_RELU_MAX)
+    return z != z ? make_float2(z, z) : z > 0.0f ? make_float2(z, 1.0f) : make_float2(0.0f, 0.0f);
+  if constexpr (ACT == BGNN_ACT_ELU) {
+    const float e = p * expm1f(z);
+    return z > 0.0f ? make_float2(z, 1.0f) : make_float2(e, e + p);
+  }
+  if constexpr (ACT == BGNN_ACT_LEAKY_RELU)
+    return z > 0.0f ? make_float2(z, 1.0f) : make_float2(p * z, p);
+  if constexpr (ACT == BGNN_ACT_SIGMOID) {
+    const float g = sigmoid_t(-LOG2E * z);
+    return make_float2(g, g * sigmoid_t(LOG2E * z));
+  }
+  if constexpr (ACT == BGNN_ACT_TANH) {
+    const float t = tanhf(z);
+    return make_float2(t, (1.0f - t) * (1.0f + t));
+  }
+  return make_float2(z, 1.0f);
+}
+template <int ACT>
+__device__ __forceinline__ void act_grad_two(float z0, float z1, float p, float2& f0, float2& f1) {
+  float2 s = make_float2(0.0f, 0.0f);
+  if constexpr (GATES<ACT>) s = sigmoid_t2(gate_t<ACT>(z0), gate_t<ACT>(z1));
+  f0 = act_grad<ACT>(z0, s.x, p);
+  f1 = act_grad<ACT>(z1, s.y, p);
+}
+// Runs f(Act<..>) for an activation known at run time.  One branch a chunk of
+// 32 elements: the switch inside the element loop made the code of every
+// activation part of every element (7.8 ms instead of 1.x at 2.45M x 256 -> 512).
+template <int ACT>
+using Act = std::integral_constant<int, ACT>;
+template <class F>
+__device__ __forceinline__ void with_act(int act, F&& f) {
   switch (act) {
-    case BGNN_ACT_RELU: return z > 0.0f ? make_float2(z, 1.0f) : make_float2(0.0f, 0.0f);
-    case BGNN_ACT_RELU_MAX:
-      return z != z ? make_float2(z, z) : z > 0.0f ? make_float2(z, 1.0f) : make_float2(0.0f, 0.0f);
-    case BGNN_ACT_ELU: {
-      const float e = p * expm1f(z);
-      return z > 0.0f ? make_float2(z, 1.0f) : make_float2(e, e + p);
-    }
-    case BGNN_ACT_LEAKY_RELU: return z > 0.0f ? make_float2(z, 1.0f) : make_float2(p * z, p);
-    case BGNN_ACT_SIGMOID: {
-      const float s = sigmoid_f(z);
-      return make_float2(s, s * sigmoid_f(-z));
-    }
-    case BGNN_ACT_TANH: {
-      const float t = tanhf(z);
-      return make_float2(t, (1.0f - t) * (1.0f + t));
-    }
-    case BGNN_ACT_GELU: {
-      const float s = sigmoid_f(2.0f * gelu_arg(z));
-      const float dv = 2.0f * GELU_C * fmaf(3.0f * 0.044715f * z, z, 1.0f);
-      // far out s is 0 or 1 and z (1 - s) 0, whatever dv is
-      const float q = s * (1.0f - s);
-      return make_float2(z * s, q == 0.0f ? s : fmaf(z * q, dv, s));
-    }
-    case BGNN_ACT_SILU: {
-      const float s = sigmoid_f(z);
-      return make_float2(z * s, s * fmaf(z, 1.0f - s, 1.0f));
-    }
-    default: return make_float2(z, 1.0f);
+    case BGNN_ACT_RELU: f(Act<BGNN_ACT_RELU>{}); break;
+    case BGNN_ACT_RELU_MAX: f(Act<BGNN_ACT_RELU_MAX>{}); break;
+    case BGNN_ACT_ELU: f(Act<BGNN_ACT_ELU>{}); break;
+    case BGNN_ACT_LEAKY_RELU: f(Act<BGNN_ACT_LEAKY_RELU>{}); break;
+    case BGNN_ACT_SIGMOID: f(Act<BGNN_ACT_SIGMOID>{}); break;
+    case BGNN_ACT_TANH: f(Act<BGNN_ACT_TANH>{}); break;
+    case BGNN_ACT_GELU: f(Act<BGNN_ACT_GELU>{}); break;
+    case BGNN_ACT_SILU: f(Act<BGNN_ACT_SILU>{}); break;
+    default: f(Act<BGNN_ACT_NONE>{}); break;
   }
 }
 
-// ---- the turning buffer: 32 rows x 32 f32, 16-byte units swizzled by row --------
-__device__ __forceinline__ float4* turn_unit(float* t, int row, int unit) {
-  return reinterpret_cast<float4*>(t + row * 32 + ((unit ^ (row & 7)) << 2));
+// ---- chunk slots: 32 rows of 128 bytes (f32) or 64 bytes (16 bits), 16-byte
+// units swizzled as TMA does, so that a row a lane has no bank conflicts ---------
+__device__ __forceinline__ float4* turn_unit(void* slot, int row, int unit) {
+  return reinterpret_cast<float4*>(static_cast<char*>(slot) + row * 128 +
+                                   ((unit ^ (row & 7)) << 4));
 }
-__device__ __forceinline__ void turn_put_row(float* t, int row, const float (&v)[32]) {
+__device__ __forceinline__ uint4* turn_unit16(void* slot, int row, int unit) {
+  return reinterpret_cast<uint4*>(static_cast<char*>(slot) + row * 64 +
+                                  ((unit ^ ((row >> 1) & 3)) << 4));
+}
+template <int DT>
+__device__ __forceinline__ void put_row16(void* slot, int row, const float (&v)[32]) {
 #pragma unroll
-  for (int u = 0; u < 8; u++)
-    *turn_unit(t, row, u) = make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+  for (int u = 0; u < 4; u++)
+    *turn_unit16(slot, row, u) =
+        make_uint4(pack2<DT>(v[8 * u], v[8 * u + 1]), pack2<DT>(v[8 * u + 2], v[8 * u + 3]),
+                   pack2<DT>(v[8 * u + 4], v[8 * u + 5]), pack2<DT>(v[8 * u + 6], v[8 * u + 7]));
+}
+// a row of a chunk into a slot, rounded to the element type
+__device__ __forceinline__ void put_row(void* slot, int row, int dt, const float (&v)[32]) {
+  if (dt == BGNN_F32) {
+#pragma unroll
+    for (int u = 0; u < 8; u++)
+      *turn_unit(slot, row, u) = make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+  } else if (dt == BGNN_BF16) {
+    put_row16<BGNN_BF16>(slot, row, v);
+  } else {
+    put_row16<BGNN_F16>(slot, row, v);
+  }
+}
+// a row of a slot: f(i, value) for its 32 elements
+template <class F>
+__device__ __forceinline__ void each_of_row(void* slot, int row, int dt, F&& f) {
+  if (dt == BGNN_F32) {
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      const float4 w = *turn_unit(slot, row, u);
+      f(4 * u, w.x), f(4 * u + 1, w.y), f(4 * u + 2, w.z), f(4 * u + 3, w.w);
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const uint4 q = *turn_unit16(slot, row, u);
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        if (dt == BGNN_BF16) {
+          f(8 * u + 2 * i, __uint_as_float(w[i] << 16));
+          f(8 * u + 2 * i + 1, __uint_as_float(w[i] & 0xffff0000u));
+        } else {
+          const float2 q2 = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          f(8 * u + 2 * i, q2.x);
+          f(8 * u + 2 * i + 1, q2.y);
+        }
+      }
+    }
+  }
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, uint32_t src) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+          reinterpret_cast<uint64_t>(map)),
+      "r"(x), "r"(y), "r"(src)
+      : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// all but N of this thread's stores have read their shared memory
+template <int N>
+__device__ __forceinline__ void stores_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+// this thread's stores are done
+__device__ __forceinline__ void stores_done() {
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+__device__ __forceinline__ void fence_async() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
 // four consecutive elements along a row, or those of them that exist
@@ -312,20 +554,20 @@ __device__ __forceinline__ bool vec4_ok(const void* p, int dt, uint64_t ld) {
 struct Tile {
   uint32_t m0, n0, batch, split;
 };
-template <int EPI>
+template <int EPI, int CG>
 __device__ __forceinline__ Tile tile_at(const GemmArgs& g, uint64_t t, uint32_t n_tiles,
                                         uint32_t m_tiles, uint32_t wn) {
   Tile r;
   const uint64_t q = t / n_tiles;
   r.n0 = (uint32_t)(t % n_tiles) * wn;
-  r.m0 = (uint32_t)(q % m_tiles) * BM;
+  r.m0 = (uint32_t)(q % m_tiles) * (BM * CG);
   const uint32_t z = (uint32_t)(q / m_tiles);
   r.batch = EPI == EPI_PARTIAL ? z % g.batches : 0;
   r.split = EPI == EPI_PARTIAL ? z / g.batches : 0;
   return r;
 }
 
-template <int EPI>
+template <int EPI, int CG>
 __global__ void __launch_bounds__(THREADS, 1)
     k_dense16(const __grid_constant__ Maps maps, const GemmArgs g) {
   constexpr bool TWO = EPI == EPI_GATED || EPI == EPI_GATED_BWD;  // B tile of two weights
@@ -333,15 +575,16 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t raw = s_addr(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;  // swizzle atoms start on 1024 bytes
   uint8_t* gbase = smem_raw + (base - raw);
-  float* turns = reinterpret_cast<float*>(gbase + RING_BYTES);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(gbase + RING_BYTES + EPI_WARPS * TURN_BYTES);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(gbase + RING_BYTES + EPI_WARPS * WARP_BYTES);
   const uint32_t b_full = s_addr(bars), b_empty = b_full + 8 * MAX_STAGES;
-  const uint32_t b_accf = b_empty + 8 * MAX_STAGES, b_acce = b_accf + 16, b_last = b_acce + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * MAX_STAGES + 5);
+  const uint32_t b_accf = b_empty + 8 * MAX_STAGES, b_acce = b_accf + 16, b_in = b_acce + 16;
+  const uint32_t b_last = b_in + 8 * EPI_WARPS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * MAX_STAGES + 4 + EPI_WARPS + 1);
   volatile uint32_t* abort_flag = tmem_slot + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? cta_rank() : 0u;  // of the pair; rank 0 issues the products
   const uint32_t S = g.stages;
-  const uint32_t tmem_cols = 2 * g.bn < 32 ? 32 : 2 * g.bn;
+  const uint32_t tmem_cols = 2 * g.bn;
 
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < S; s++) {
@@ -350,28 +593,27 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     for (int b = 0; b < 2; b++) {
       mbar_init(b_accf + 8 * b, 1);
-      mbar_init(b_acce + 8 * b, EPI_WARPS * 32);
+      mbar_init(b_acce + 8 * b, EPI_WARPS * CG);
     }
+    for (int w = 0; w < EPI_WARPS; w++) mbar_init(b_in + 8 * w, 1);
     mbar_init(b_last, 1);
     *abort_flag = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == EPI_WARPS) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     s_addr(tmem_slot)),
-                 "r"(tmem_cols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tmem_alloc<CG>(s_addr(tmem_slot), tmem_cols);
     tc_fence_before();
   }
-  __syncthreads();
+  pair_sync<CG>();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
   const uint32_t wn = TWO ? g.bn / 2 : g.bn;  // output columns of a tile
-  const uint32_t m_tiles = (g.m + BM - 1) / BM, n_tiles = (g.n + wn - 1) / wn;
+  const uint32_t bl = g.bn / CG;              // rows of the B tile that this CTA loads
+  const uint32_t n_tiles = (g.n + wn - 1) / wn, m_tiles = (g.m + BM * CG - 1) / (BM * CG);
   const uint64_t tiles = (uint64_t)m_tiles * n_tiles *
                          (EPI == EPI_PARTIAL ? (uint64_t)g.batches * g.splits : 1ull);
+  const uint64_t t_first = blockIdx.x / CG, t_step = gridDim.x / CG;
   const uint32_t nkb = g.nkb[0] + g.nkb[1];
   // k blocks [first, last) of a tile
   auto kb_first = [&](const Tile& t) { return EPI == EPI_PARTIAL ? t.split * g.per : 0u; };
@@ -386,232 +628,347 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (lane == 0) {
       uint32_t s = 0, ph = 0;
       uint64_t filled = 0;
-      const uint32_t tx = A_BYTES + g.bn * 128;
+      const uint32_t tx = CG * (A_BYTES + bl * 128);
       const int kw = g.fp8 ? 128 : 64;  // elements of a k block
-      for (uint64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-        const Tile ti = tile_at<EPI>(g, t, n_tiles, m_tiles, wn);
+      for (uint64_t t = t_first; t < tiles; t += t_step) {
+        const Tile ti = tile_at<EPI, CG>(g, t, n_tiles, m_tiles, wn);
+        const int am = (int)(ti.m0 + rank * BM);
         const uint32_t e = kb_last(ti);
         for (uint32_t kb = kb_first(ti); kb < e; kb++) {
           if (!mbar_wait(b_empty + 8 * s, ph ^ 1u, abort_flag, g.err, 70)) goto drain;
-          mbar_expect_tx(b_full + 8 * s, tx);
+          if (rank == 0) mbar_expect_tx(b_full + 8 * s, tx);
           const int seg = EPI == EPI_PARTIAL ? (int)ti.batch : (kb >= g.nkb[0] ? 1 : 0);
           const int k0 = (int)((EPI != EPI_PARTIAL && seg ? kb - g.nkb[0] : kb)) * kw;
-          const uint32_t st = base + s * g.stage_bytes, bar = b_full + 8 * s;
+          const uint32_t st = base + s * g.stage_bytes;
+          // both CTAs' loads count on the issuing CTA's barrier
+          const uint32_t bar = CG == 2 ? peer_addr(b_full + 8 * s, 0) : b_full + 8 * s;
           if (g.a_mn) {
             for (int i = 0; i < BM / 64; i++)
-              tma_load_2d(st + i * 8192, &maps.a[seg], (int)ti.m0 + i * 64, k0, bar);
+              tma_load_2d<CG>(st + i * 8192, &maps.a[seg], am + i * 64, k0, bar);
           } else {
-            tma_load_2d(st, &maps.a[seg], k0, (int)ti.m0, bar);
+            tma_load_2d<CG>(st, &maps.a[seg], k0, am, bar);
           }
-          if (TWO) {
-            tma_load_2d(st + A_BYTES, &maps.b[0], k0, (int)ti.n0, bar);
-            tma_load_2d(st + A_BYTES + wn * 128, &maps.b[1], k0, (int)ti.n0, bar);
-          } else if (g.b_mn) {
-            const CUtensorMap* mb = EPI == EPI_PARTIAL ? &maps.b[0] : &maps.b[seg];
-            for (uint32_t i = 0; i < g.bn / 64; i++)
-              tma_load_2d(st + A_BYTES + i * 8192, mb, (int)(ti.n0 + i * 64), k0, bar);
+          if (TWO && CG == 2) {  // one weight a CTA
+            tma_load_2d<CG>(st + A_BYTES, &maps.b[rank], k0, (int)ti.n0, bar);
+          } else if (TWO) {
+            tma_load_2d<CG>(st + A_BYTES, &maps.b[0], k0, (int)ti.n0, bar);
+            tma_load_2d<CG>(st + A_BYTES + wn * 128, &maps.b[1], k0, (int)ti.n0, bar);
           } else {
-            tma_load_2d(st + A_BYTES, &maps.b[seg], k0, (int)ti.n0, bar);
+            const CUtensorMap* mb = EPI == EPI_PARTIAL ? &maps.b[0] : &maps.b[seg];
+            const int bn0 = (int)(ti.n0 + rank * bl);
+            if (g.b_mn) {
+              for (uint32_t i = 0; i < bl / 64; i++)
+                tma_load_2d<CG>(st + A_BYTES + i * 8192, mb, bn0 + (int)i * 64, k0, bar);
+            } else {
+              tma_load_2d<CG>(st + A_BYTES, mb, k0, bn0, bar);
+            }
           }
           filled++;
           if (++s == S) s = 0, ph ^= 1u;
         }
       }
     drain:
-      if (*abort_flag)  // the last fill of every stage lands before the CTA ends
+      if (*abort_flag && rank == 0)  // the last fill of every stage lands before the CTA ends
         for (uint64_t f = filled > S ? filled - S : 0; f < filled; f++)
           mbar_drain(b_full + 8 * (uint32_t)(f % S), (uint32_t)((f / S) & 1u));
     }
   } else if (warp == EPI_WARPS + 1) {
     // ---- MMA issuer ----
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       uint32_t s = 0, ph = 0, buf = 0, aph = 0;
       const uint32_t step_a = g.a_mn ? 2048u : 32u, step_b = g.b_mn ? 2048u : 32u;
-      for (uint64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-        const Tile ti = tile_at<EPI>(g, t, n_tiles, m_tiles, wn);
-        const uint32_t f = kb_first(ti), e = kb_last(ti);
-        if (!mbar_wait(b_acce + 8 * buf, aph ^ 1u, abort_flag, g.err, 71)) break;
-        tc_fence_after();
-        const uint32_t d = tmem + buf * g.bn;
-        bool gave_up = false;
-        for (uint32_t kb = f; kb < e; kb++) {
-          if (!mbar_wait(b_full + 8 * s, ph, abort_flag, g.err, 72)) {
-            gave_up = true;
-            break;
-          }
+      for (uint64_t t = t_first; t < tiles; t += t_step) {
+        const Tile ti = tile_at<EPI, CG>(g, t, n_tiles, m_tiles, wn);
+        const uint32_t last = kb_last(ti);
+        uint32_t kb = kb_first(ti);
+        do {  // a piece of the contraction into one accumulator
+          const uint32_t e = EPI == EPI_LINEAR_F32 && last - kb > PIECE ? kb + PIECE : last;
+          if (!mbar_wait(b_acce + 8 * buf, aph ^ 1u, abort_flag, g.err, 71)) goto stop;
           tc_fence_after();
-          const uint32_t st = base + s * g.stage_bytes;
+          const uint32_t d = tmem + buf * g.bn;
+          uint32_t acc = 0u;
+          for (; kb < e; kb++) {
+            if (!mbar_wait(b_full + 8 * s, ph, abort_flag, g.err, 72)) goto stop;
+            tc_fence_after();
+            const uint32_t st = base + s * g.stage_bytes;
 #pragma unroll
-          for (uint32_t kk = 0; kk < 4; kk++) {
-            const uint64_t da = smem_desc(st + kk * step_a, g.a_mn);
-            const uint64_t db = smem_desc(st + A_BYTES + kk * step_b, g.b_mn);
-            const uint32_t acc = (kb != f || kk != 0) ? 1u : 0u;
-            if (g.fp8) mma_f8(d, da, db, g.idesc, acc);
-            else mma_f16(d, da, db, g.idesc, acc);
+            for (uint32_t kk = 0; kk < 4; kk++) {
+              const uint64_t da = smem_desc(st + kk * step_a, g.a_mn);
+              const uint64_t db = smem_desc(st + A_BYTES + kk * step_b, g.b_mn);
+              if (g.fp8) mma_f8<CG>(d, da, db, g.idesc, acc);
+              else mma_f16<CG>(d, da, db, g.idesc, acc);
+              acc = 1u;
+            }
+            mma_commit<CG>(b_empty + 8 * s);
+            if (++s == S) s = 0, ph ^= 1u;
           }
-          mma_commit(b_empty + 8 * s);
-          if (++s == S) s = 0, ph ^= 1u;
-        }
-        if (gave_up) break;
-        mma_commit(b_accf + 8 * buf);
-        if (++buf == 2) buf = 0, aph ^= 1u;
+          mma_commit<CG>(b_accf + 8 * buf);
+          if (++buf == 2) buf = 0, aph ^= 1u;
+        } while (kb < last);
       }
+    stop:
       // every product issued is done before tensor memory is freed
-      mma_commit(b_last);
+      mma_commit_here<CG>(b_last);
       mbar_drain(b_last, 0);
     }
   } else {
     // ---- epilogue ----
     const int quad = warp & 3, half = warp >> 2;
-    float* turn = turns + warp * (TURN_BYTES / 4);
-    uint32_t buf = 0, aph = 0;
-    const bool vec_out = EPI == EPI_PARTIAL ? g.n % 4 == 0
-                                            : vec4_ok(g.out[0], g.out_type, g.ld_out) &&
-                                                  (EPI != EPI_GATED_BWD ||
-                                                   vec4_ok(g.out[1], g.out_type, g.ld_out));
+    uint8_t* in_slot = gbase + RING_BYTES + warp * WARP_BYTES;
+    uint8_t* out_slot = in_slot + SLOT_BYTES;  // one f32 chunk, or two 16-bit ones in turn
+    const uint32_t in_bar = b_in + 8 * warp;
+    uint32_t buf = 0, aph = 0, in_ph = 0, out_at = 0;
+    const bool parts = EPI == EPI_PARTIAL && g.part_rows;
+    const bool vec_out = vec4_ok(g.out[0], g.out_type, g.ld_out) &&
+                         (!g.out[1] || vec4_ok(g.out[1], g.out_type, g.ld_out));
     const bool vec_other = g.other && vec4_ok(g.other, g.other_type, g.ld_other);
-    for (uint64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-      const Tile ti = tile_at<EPI>(g, t, n_tiles, m_tiles, wn);
-      const bool any_k = kb_first(ti) < kb_last(ti);
-      if (!mbar_wait(b_accf + 8 * buf, aph, abort_flag, g.err, 73)) break;
-      tc_fence_after();
-      const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + buf * g.bn;
-      const uint32_t row0 = ti.m0 + quad * 32;  // this warp's rows
+    const uint32_t in_bytes = g.other_type == BGNN_F32 ? 4096u : 2048u;
+    // hands the accumulator back once every lane has read it
+    auto release = [&]() {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_at<CG>(b_acce + 8 * buf);
+      if (++buf == 2) buf = 0, aph ^= 1u;
+    };
+    bool gave_up = false;
+    for (uint64_t t = t_first; t < tiles && !gave_up; t += t_step) {
+      const Tile ti = tile_at<EPI, CG>(g, t, n_tiles, m_tiles, wn);
+      const uint32_t k_first = kb_first(ti), k_last = kb_last(ti);
+      const bool any_k = k_first < k_last;
+      const uint32_t row0 = ti.m0 + rank * BM + quad * 32;  // this warp's rows
       const float xs = g.x_scale && row0 + lane < g.m ? g.x_scale[row0 + lane] : 1.0f;
-      for (uint32_t c = half * 32; c < wn; c += 64) {
-        const uint32_t col0 = ti.n0 + c;
-        if (col0 >= g.n) break;  // uniform: the chunk is past the last column
-        float v[32];
-        tmem_ld32(acc + c, v);
-        if (!any_k) {
-#pragma unroll
-          for (int j = 0; j < 32; j++) v[j] = 0.0f;
+      const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+      // asks for the chunk of the residual / upstream gradient at col0; every
+      // lane is done with the one before
+      auto ask = [&](uint32_t col0) {
+        if (lane == 0) {
+          fence_async();
+          mbar_expect_tx(in_bar, in_bytes);
+          tma_load_2d<1>(s_addr(in_slot), &maps.in, (int)col0, (int)row0, in_bar);
         }
-        if constexpr (EPI != EPI_PARTIAL) {
-          if (g.x_scale) {
-#pragma unroll
-            for (int j = 0; j < 32; j++)
-              v[j] *= xs * (col0 + j < g.n ? g.w_scale[0][col0 + j] : 0.0f);
-          }
-          if (g.bias[0]) {
-#pragma unroll
-            for (int j = 0; j < 32; j++)
-              if (col0 + j < g.n) v[j] += load_any(g.bias[0], g.bias_type, col0 + j);
-          }
-        }
-        // the upstream gradient of this chunk, read along rows
-        auto other_rows = [&](float (&o)[32]) {
+      };
+      if (g.tma_in && ti.n0 + half * 32 < g.n && half * 32 < wn) ask(ti.n0 + half * 32);
+      // f(j, value) over this lane's row of the chunk at col0; `next` is the
+      // chunk after it (or >= g.n)
+      auto take = [&](uint32_t col0, uint32_t next, auto f) {
+        if (g.tma_in) {
+          if (!mbar_wait(in_bar, in_ph, abort_flag, g.err, 74)) gave_up = true;
+          in_ph ^= 1u;
+          each_of_row(in_slot, lane, g.other_type, f);
           __syncwarp();
+          if (next < g.n) ask(next);
+        } else {  // rows that TMA cannot take: plain reads along rows, turned round
+          float4 w[8];
+#pragma unroll
           for (int i = 0; i < 8; i++) {
             const int r = i * 4 + (lane >> 3), u = lane & 7;
             const uint32_t row = row0 + r, col = col0 + u * 4;
-            float4 w = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            w[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (row < g.m && col < g.n)
-              w = load4_row(g.other, g.other_type, (uint64_t)row * g.ld_other + col, g.n - col,
-                            vec_other);
-            *turn_unit(turn, r, u) = w;
+              w[i] = load4_row(g.other, g.other_type, (uint64_t)row * g.ld_other + col, g.n - col,
+                               vec_other);
           }
           __syncwarp();
 #pragma unroll
-          for (int u = 0; u < 8; u++) {
-            const float4 w = *turn_unit(turn, lane, u);
-            o[4 * u] = w.x, o[4 * u + 1] = w.y, o[4 * u + 2] = w.z, o[4 * u + 3] = w.w;
+          for (int i = 0; i < 8; i++) *turn_unit(in_slot, i * 4 + (lane >> 3), lane & 7) = w[i];
+          __syncwarp();
+          each_of_row(in_slot, lane, BGNN_F32, f);
+        }
+      };
+      // a chunk out, a row a lane
+      auto give = [&](const float (&v)[32], uint32_t col0, int which, int type, uint32_t out_row) {
+        if (g.tma_out) {
+          uint8_t* slot = out_slot;
+          if (type != BGNN_F32) {
+            slot += out_at * 2048;
+            out_at ^= 1u;
+            if (lane == 0) stores_read<1>();
+          } else {
+            if (lane == 0) stores_read<0>();
           }
-        };
-        // v (a row a lane) out along rows; with_other: add the residual on the way
-        auto rows_out = [&](void* out, int out_type, uint64_t ld, bool with_other) {
           __syncwarp();
-          turn_put_row(turn, lane, v);
+          put_row(slot, lane, type, v);
+          fence_async();
           __syncwarp();
+          if (lane == 0 && row0 < g.m)
+            tma_store_2d(&maps.out[which], (int)col0, (int)out_row, s_addr(slot));
+        } else {
+          __syncwarp();
+          put_row(out_slot, lane, BGNN_F32, v);
+          __syncwarp();
+#pragma unroll
           for (int i = 0; i < 8; i++) {
             const int r = i * 4 + (lane >> 3), u = lane & 7;
             const uint32_t row = row0 + r, col = col0 + u * 4;
-            if (row < g.m && col < g.n) {
-              float4 w = *turn_unit(turn, r, u);
-              if (with_other) {
-                const float4 q = load4_row(g.other, g.other_type,
-                                           (uint64_t)row * g.ld_other + col, g.n - col, vec_other);
-                w.x += q.x, w.y += q.y, w.z += q.z, w.w += q.w;
-              }
-              store4_row(out, out_type, (uint64_t)row * ld + col, g.n - col, vec_out, w);
+            if (row < g.m && col < g.n)
+              store4_row(g.out[which], type, (uint64_t)row * g.ld_out + col, g.n - col, vec_out,
+                         *turn_unit(out_slot, r, u));
+          }
+        }
+      };
+      // scales and bias of a chunk: lane j holds column j's
+      auto scaled = [&](float (&v)[32], uint32_t col0, int i) {
+        const bool in = col0 + lane < g.n;
+        if (g.x_scale) {
+          const float ws = in ? g.w_scale[i][col0 + lane] : 0.0f;
+#pragma unroll
+          for (int j = 0; j < 32; j++) v[j] *= xs * __shfl_sync(0xffffffffu, ws, j);
+        }
+        if (g.bias[i]) {
+          const float bv = in ? load_any(g.bias[i], g.bias_type, col0 + lane) : 0.0f;
+#pragma unroll
+          for (int j = 0; j < 32; j++) v[j] += __shfl_sync(0xffffffffu, bv, j);
+        }
+      };
+      auto linear_out = [&](float (&v)[32], uint32_t col0, uint32_t next) {
+        scaled(v, col0, 0);
+        if (g.act != BGNN_ACT_NONE)
+          with_act(g.act, [&](auto act) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 2)
+              act_two<decltype(act)::value>(v[j], v[j + 1], g.act_p);
+          });
+        if (g.other) take(col0, next, [&](int j, float o) { v[j] += o; });
+        give(v, col0, 0, g.out_type, row0);
+      };
+      auto after = [&](uint32_t c) { return c + 64 < wn ? ti.n0 + c + 64 : g.n; };
+
+      if constexpr (EPI == EPI_LINEAR_F32) {
+        // pieces of the contraction added in f32 registers, rounded to nearest
+        float sum[4][32];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int j = 0; j < 32; j++) sum[i][j] = 0.0f;
+        uint32_t kb = k_first;
+        do {
+          if (!mbar_wait(b_accf + 8 * buf, aph, abort_flag, g.err, 73)) {
+            gave_up = true;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t acc = tmem + lanes + buf * g.bn;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const uint32_t c = half * 32 + i * 64;
+            if (c < wn && any_k) {
+              float v[32];
+              tmem_ld32(acc + c, v);
+              tmem_wait_ld(v);
+#pragma unroll
+              for (int j = 0; j < 32; j++) sum[i][j] += v[j];
             }
           }
-        };
-        if constexpr (EPI == EPI_LINEAR) {
-          if (g.act != BGNN_ACT_NONE) {
+          release();
+          kb += PIECE;
+        } while (kb < k_last);
+        if (gave_up) break;
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = act_f(v[j], g.act, g.act_p);
-          }
-          rows_out(g.out[0], g.out_type, g.ld_out, g.other != nullptr);
-        } else if constexpr (EPI == EPI_PARTIAL) {
-          rows_out(g.part + ((uint64_t)ti.split * g.batches + ti.batch) * g.m * g.n, BGNN_F32, g.n,
-                   false);
-        } else if constexpr (EPI == EPI_LINEAR_BWD) {
-          float o[32];
-          other_rows(o);
-#pragma unroll
-          for (int j = 0; j < 32; j++) v[j] = o[j] * act_both(v[j], g.act, g.act_p).y;
-          rows_out(g.out[0], g.out_type, g.ld_out, false);
-        } else {
-          float u[32];
-          tmem_ld32(acc + wn + c, u);
+        for (int i = 0; i < 4; i++) {
+          const uint32_t c = half * 32 + i * 64;
+          if (c < wn && ti.n0 + c < g.n) linear_out(sum[i], ti.n0 + c, after(c));
+        }
+      } else {
+        if (!mbar_wait(b_accf + 8 * buf, aph, abort_flag, g.err, 73)) break;
+        tc_fence_after();
+        const uint32_t acc = tmem + lanes + buf * g.bn;
+        for (uint32_t c = half * 32; c < wn; c += 64) {
+          const uint32_t col0 = ti.n0 + c;
+          if (col0 >= g.n) break;  // uniform: the chunk is past the last column
+          float v[32], u[32];      // u: the second product's
+          tmem_ld32(acc + c, v);
+          if constexpr (TWO) tmem_ld32(acc + wn + c, u);
+          tmem_wait_ld(v);
+          if constexpr (TWO) tmem_wait_ld(u);
           if (!any_k) {
 #pragma unroll
-            for (int j = 0; j < 32; j++) u[j] = 0.0f;
-          }
-          if (g.x_scale) {
-#pragma unroll
-            for (int j = 0; j < 32; j++)
-              u[j] *= xs * (col0 + j < g.n ? g.w_scale[1][col0 + j] : 0.0f);
-          }
-          if (g.bias[1]) {
-#pragma unroll
-            for (int j = 0; j < 32; j++)
-              if (col0 + j < g.n) u[j] += load_any(g.bias[1], g.bias_type, col0 + j);
-          }
-          if constexpr (EPI == EPI_GATED) {
-#pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = act_f(v[j], g.act, g.act_p) * u[j];
-            rows_out(g.out[0], g.out_type, g.ld_out, false);
-          } else {
-            float o[32];
-            other_rows(o);
-#pragma unroll
             for (int j = 0; j < 32; j++) {
-              const float2 f = act_both(v[j], g.act, g.act_p);
-              v[j] = o[j] * u[j] * f.y;  // dg
-              u[j] = o[j] * f.x;         // du
+              v[j] = 0.0f;
+              if constexpr (TWO) u[j] = 0.0f;
             }
-            rows_out(g.out[0], g.out_type, g.ld_out, false);
+          }
+          if constexpr (EPI == EPI_LINEAR) {
+            linear_out(v, col0, after(c));
+          } else if constexpr (EPI == EPI_PARTIAL) {
+            if (parts)
+              give(v, col0, 0, BGNN_F32,
+                   row0 + (ti.split * g.batches + ti.batch) * g.part_rows);
+            else
+              give(v, col0, (int)ti.batch, g.out_type, row0);
+          } else if constexpr (EPI == EPI_LINEAR_BWD) {
+            scaled(v, col0, 0);
+            float o[32];
+            take(col0, after(c), [&](int j, float w) { o[j] = w; });
+            with_act(g.act, [&](auto act) {
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = u[j];
-            rows_out(g.out[1], g.out_type, g.ld_out, false);
+              for (int j = 0; j < 32; j += 2) {
+                float2 f0, f1;
+                act_grad_two<decltype(act)::value>(v[j], v[j + 1], g.act_p, f0, f1);
+                v[j] = o[j] * f0.y;
+                v[j + 1] = o[j + 1] * f1.y;
+              }
+            });
+            give(v, col0, 0, g.out_type, row0);
+          } else if constexpr (EPI == EPI_GATED) {
+            scaled(v, col0, 0);
+            scaled(u, col0, 1);
+            with_act(g.act, [&](auto act) {
+#pragma unroll
+              for (int j = 0; j < 32; j += 2) {
+                act_two<decltype(act)::value>(v[j], v[j + 1], g.act_p);
+                v[j] *= u[j];
+                v[j + 1] *= u[j + 1];
+              }
+            });
+            give(v, col0, 0, g.out_type, row0);
+          } else {
+            scaled(v, col0, 0);
+            scaled(u, col0, 1);
+            float o[32];
+            take(col0, after(c), [&](int j, float w) { o[j] = w; });
+            with_act(g.act, [&](auto act) {
+#pragma unroll
+              for (int j = 0; j < 32; j += 2) {
+                float2 f0, f1;
+                act_grad_two<decltype(act)::value>(v[j], v[j + 1], g.act_p, f0, f1);
+                v[j] = o[j] * u[j] * f0.y;  // dg
+                v[j + 1] = o[j + 1] * u[j + 1] * f1.y;
+                u[j] = o[j] * f0.x;  // du
+                u[j + 1] = o[j + 1] * f1.x;
+              }
+            });
+            give(v, col0, 0, g.out_type, row0);
+            give(u, col0, 1, g.out_type, row0);
           }
         }
+        release();
       }
-      tc_fence_before();
-      mbar_arrive(b_acce + 8 * buf);
-      if (++buf == 2) buf = 0, aph ^= 1u;
     }
+    if (lane == 0) stores_done();
   }
-  __syncthreads();
+  pair_sync<CG>();
   if (warp == EPI_WARPS) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols)
-                 : "memory");
+    tmem_free<CG>(tmem, tmem_cols);
   }
 }
 
-// dw: the splits' partial tiles added in order
-__global__ void __launch_bounds__(256) k_add_splits(const float* __restrict__ part,
-                                                    uint32_t splits, uint32_t batches, uint64_t mn,
-                                                    void* out0, void* out1, int out_type) {
-  const uint64_t total = mn * batches;
+// dw: the splits' partial matrices (prows rows of ld f32 each) added in order
+__global__ void __launch_bounds__(256) k_add_splits(const float* __restrict__ part, uint32_t splits,
+                                                    uint32_t batches, uint32_t prows, uint32_t ld,
+                                                    uint32_t rows, uint32_t cols, void* out0,
+                                                    void* out1, int out_type) {
+  const uint64_t mn = (uint64_t)rows * cols, total = mn * batches;
+  const uint64_t step = (uint64_t)prows * ld * batches;
   for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
        i += (uint64_t)gridDim.x * blockDim.x) {
-    float v = part[i];
-    for (uint32_t s = 1; s < splits; s++) v += part[(uint64_t)s * total + i];
-    store_any(i < mn ? out0 : out1, out_type, i < mn ? i : i - mn, v);
+    const uint32_t b = i >= mn;
+    const uint64_t e = b ? i - mn : i;
+    const uint32_t r = (uint32_t)(e / cols), c = (uint32_t)(e - (uint64_t)r * cols);
+    const float* p = part + ((uint64_t)b * prows + r) * ld + c;
+    float v = *p;
+    for (uint32_t s = 1; s < splits; s++) v += p[s * step];
+    store_any(b ? out1 : out0, out_type, e, v);
   }
 }
 
@@ -691,11 +1048,61 @@ int make_map(bgnn_ctx* ctx, CUtensorMap* map, int type, const Mat& x, uint32_t b
   return BGNN_OK;
 }
 
+// whether TMA can take a matrix as it lies
+bool tma_takes(int type, const Mat& x) {
+  const uint64_t pitch = x.ld * dtype_size(type);
+  return ((uintptr_t)x.p & 15u) == 0 && pitch % 16 == 0 && pitch < (1ull << 40) &&
+         x.rows < (1ull << 31);
+}
+
+// 32 x 32 boxes of f32 (128-byte swizzle) or 16-bit (64-byte) elements: the
+// epilogue's chunks
+int make_chunk_map(bgnn_ctx* ctx, CUtensorMap* map, int type, const Mat& x) {
+  auto enc = encode_fn();
+  if (!enc) return bgnn_set_error(ctx, BGNN_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[2] = {x.cols, x.rows};
+  cuuint64_t strides[1] = {x.ld * dtype_size(type)};
+  cuuint32_t box[2] = {32, 32};
+  cuuint32_t el[2] = {1, 1};
+  const CUtensorMapDataType dt = type == BGNN_BF16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                 : type == BGNN_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                    : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  const CUresult r =
+      enc(map, dt, 2, const_cast<void*>(x.p), dims, strides, box, el,
+          CU_TENSOR_MAP_INTERLEAVE_NONE,
+          type == BGNN_F32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+          CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return bgnn_set_error(ctx, BGNN_ERR_UNSUPPORTED, "tensor map encode failed (%d)", (int)r);
+  return BGNN_OK;
+}
+// maps.in and maps.out of a product [m, n] where TMA can take them
+int make_chunk_maps(bgnn_ctx* ctx, Maps* maps, GemmArgs* g) {
+  g->tma_in = 0;
+  if (g->other) {
+    const Mat in = {g->other, g->m, g->n, g->ld_other};
+    if (tma_takes(g->other_type, in)) {
+      BGNN_TRY(make_chunk_map(ctx, &maps->in, g->other_type, in));
+      g->tma_in = 1;
+    }
+  }
+  g->tma_out = 1;
+  // a TMA store writes whole 16-byte units: the columns behind a row that ends
+  // inside one would be lost
+  if (g->n * dtype_size(g->out_type) % 16) g->tma_out = 0;
+  for (int i = 0; i < 2; i++)
+    if (g->out[i] && !tma_takes(g->out_type, {g->out[i], g->m, g->n, g->ld_out})) g->tma_out = 0;
+  for (int i = 0; i < 2 && g->tma_out; i++)
+    if (g->out[i])
+      BGNN_TRY(make_chunk_map(ctx, &maps->out[i], g->out_type,
+                              {g->out[i], g->m, g->n, g->ld_out}));
+  return BGNN_OK;
+}
+
 // x as TMA can read it: itself, or a copy whose rows start on 16 bytes
 int tma_ready(bgnn_ctx* ctx, int type, Mat* x, DevTmp& tmp) {
+  if (tma_takes(type, *x)) return BGNN_OK;
   const uint32_t es = (uint32_t)dtype_size(type);
-  if (((uintptr_t)x->p & 15u) == 0 && (x->ld * es) % 16 == 0 && x->ld * es < (1ull << 40))
-    return BGNN_OK;
   const uint32_t per = 16 / es;
   const uint32_t ldp = (x->cols + per - 1) / per * per;
   BGNN_TRY(bgnn_tmp_alloc(ctx, tmp, x->rows * (uint64_t)ldp * es));
@@ -716,49 +1123,77 @@ int tma_ready(bgnn_ctx* ctx, int type, Mat* x, DevTmp& tmp) {
 
 uint32_t blocks_of(uint64_t len, uint32_t per) { return (uint32_t)((len + per - 1) / per); }
 
-// Tile width: the widest that still gives every SM a tile, since a wide tile
-// reads A fewer times; a narrow output takes the narrowest that covers it.
-uint32_t pick_bn(const bgnn_ctx* ctx, uint64_t m, uint64_t n, uint64_t z, bool two, uint32_t least) {
-  uint32_t bn = 256;
-  while (bn > least) {
-    const uint64_t wn = two ? bn / 2 : bn;
-    const uint64_t tiles = ((m + BM - 1) / BM) * ((n + wn - 1) / wn) * z;
-    if (tiles >= (uint64_t)ctx->num_sms && n > wn / 2) break;
-    bn /= 2;
+// The tile of a product: its columns in tensor memory (bn) and whether a pair
+// of CTAs shares it (256 rows, each CTA loading half of B).
+struct Shape {
+  uint32_t bn;
+  int cg;
+};
+// The widest that still gives every SM (pair) a tile, since a wide tile reads
+// A fewer times and a pair reads B once for both; a narrow output takes the
+// narrowest that covers it.
+Shape pick_shape(const bgnn_ctx* ctx, uint64_t m, uint64_t n, uint64_t z, bool two,
+                 uint32_t least) {
+  const uint64_t sms = (uint64_t)ctx->num_sms;
+  Shape s = {256, 2};
+  const uint64_t wn = two ? 128 : 256;
+  if (((m + 2 * BM - 1) / (2 * BM)) * ((n + wn - 1) / wn) * z * 2 >= sms && n > wn / 2) return s;
+  s.cg = 1;
+  while (s.bn > least) {
+    const uint64_t w = two ? s.bn / 2 : s.bn;
+    if (((m + BM - 1) / BM) * ((n + w - 1) / w) * z >= sms && n > w / 2) break;
+    s.bn /= 2;
   }
-  return bn;
+  return s;
 }
 
-void set_tile(GemmArgs* g, uint32_t bn) {
-  g->bn = bn;
-  g->stage_bytes = A_BYTES + bn * 128;
+void set_tile(GemmArgs* g, const Shape& s) {
+  g->bn = s.bn;
+  g->stage_bytes = A_BYTES + s.bn / s.cg * 128;
   g->stages = RING_BYTES / g->stage_bytes;
   if (g->stages > MAX_STAGES) g->stages = MAX_STAGES;
 }
 
-// instruction descriptor: D f32, A and B of one type, majorness, N, M = 128
-uint32_t make_idesc(int type, int a_mn, int b_mn, uint32_t bn) {
+// instruction descriptor: D f32, A and B of one type, majorness, N, M
+uint32_t make_idesc(int type, int a_mn, int b_mn, const Shape& s) {
   const uint32_t f = type == BGNN_BF16 ? 1u : 0u;  // kind::f16: 0 f16, 1 bf16; f8f6f4: 0 e4m3
   return (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
-         ((bn >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+         ((s.bn >> 3) << 17) | ((uint32_t)(BM * s.cg >> 4) << 24);
+}
+
+template <int EPI, int CG>
+int launch_cg(bgnn_ctx* ctx, const Maps& maps, const GemmArgs& g, uint64_t tiles) {
+  BGNN_CUDA(ctx, cudaFuncSetAttribute(k_dense16<EPI, CG>,
+                                      cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
+  const int sms = ctx->grid_sms > 0 && ctx->grid_sms < ctx->num_sms ? ctx->grid_sms : ctx->num_sms;
+  const uint64_t most = sms / CG > 0 ? sms / CG : 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles < most ? tiles : most) * CG);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CG;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = CG == 2 ? 1 : 0;
+  BGNN_CUDA(ctx, cudaLaunchKernelEx(&cfg, k_dense16<EPI, CG>, maps, g));
+  BGNN_LAUNCHED(ctx);
+  return BGNN_OK;
 }
 
 template <int EPI>
-int launch(bgnn_ctx* ctx, const Maps& maps, GemmArgs& g) {
+int launch(bgnn_ctx* ctx, const Maps& maps, GemmArgs& g, const Shape& s) {
   constexpr bool TWO = EPI == EPI_GATED || EPI == EPI_GATED_BWD;
-  BGNN_CUDA(ctx, cudaFuncSetAttribute(k_dense16<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      SMEM_BYTES));
-  g.idesc = make_idesc(g.in_type, g.a_mn, g.b_mn, g.bn);
+  g.idesc = make_idesc(g.in_type, g.a_mn, g.b_mn, s);
   g.fp8 = g.in_type == BGNN_E4M3;
   g.err = ctx->d_err;
-  const uint32_t wn = TWO ? g.bn / 2 : g.bn;
-  const uint64_t tiles = (uint64_t)blocks_of(g.m, BM) * blocks_of(g.n, wn) *
+  const uint32_t wn = TWO ? s.bn / 2 : s.bn;
+  const uint64_t tiles = (uint64_t)blocks_of(g.m, BM * s.cg) * blocks_of(g.n, wn) *
                          (EPI == EPI_PARTIAL ? (uint64_t)g.batches * g.splits : 1ull);
-  const int sms = ctx->grid_sms > 0 && ctx->grid_sms < ctx->num_sms ? ctx->grid_sms : ctx->num_sms;
-  const unsigned grid = (unsigned)(tiles < (uint64_t)sms ? tiles : sms);
-  k_dense16<EPI><<<grid, THREADS, SMEM_BYTES, ctx->stream>>>(maps, g);
-  BGNN_LAUNCHED(ctx);
-  return BGNN_OK;
+  return s.cg == 2 ? launch_cg<EPI, 2>(ctx, maps, g, tiles) : launch_cg<EPI, 1>(ctx, maps, g, tiles);
 }
 
 // z = x w^T (one weight or two) with the epilogue of `EPI`
@@ -768,7 +1203,8 @@ int run_nt(bgnn_ctx* ctx, GemmArgs& g, Mat x, const Mat (&w)[2], uint32_t k) {
   DevTmp tx, tw[2];
   Maps maps;
   g.a_mn = g.b_mn = 0;
-  set_tile(&g, pick_bn(ctx, g.m, g.n, 1, TWO, TWO ? 64 : 32));
+  const Shape sh = pick_shape(ctx, g.m, g.n, 1, TWO, TWO ? 64 : 32);
+  set_tile(&g, sh);
   g.nkb[0] = blocks_of(k, g.in_type == BGNN_E4M3 ? 128 : 64);
   g.nkb[1] = 0;
   if (k) {
@@ -777,10 +1213,13 @@ int run_nt(bgnn_ctx* ctx, GemmArgs& g, Mat x, const Mat (&w)[2], uint32_t k) {
     for (int i = 0; i < (TWO ? 2 : 1); i++) {
       Mat wi = w[i];
       BGNN_TRY(tma_ready(ctx, g.in_type, &wi, tw[i]));
-      BGNN_TRY(make_map(ctx, &maps.b[i], g.in_type, wi, TWO ? g.bn / 2 : g.bn));
+      BGNN_TRY(make_map(ctx, &maps.b[i], g.in_type, wi, TWO ? g.bn / 2 : g.bn / sh.cg));
     }
   }
-  return launch<EPI>(ctx, maps, g);
+  BGNN_TRY(make_chunk_maps(ctx, &maps, &g));
+  if constexpr (EPI == EPI_LINEAR)
+    if (g.out_type == BGNN_F32) return launch<EPI_LINEAR_F32>(ctx, maps, g, sh);
+  return launch<EPI>(ctx, maps, g, sh);
 }
 
 // dx = dz0 w0 (+ dz1 w1): contraction over the rows of w
@@ -794,7 +1233,8 @@ int run_dx(bgnn_ctx* ctx, int type, uint32_t m, uint32_t n, uint32_t k, const Ma
   g.in_type = type;
   g.a_mn = 0;
   g.b_mn = 1;
-  set_tile(&g, pick_bn(ctx, m, k, 1, false, 64));
+  const Shape sh = pick_shape(ctx, m, k, 1, false, 64);
+  set_tile(&g, sh);
   for (int i = 0; i < terms; i++) {
     Mat a = dz[i], b = w[i];
     g.nkb[i] = blocks_of(n, 64);
@@ -807,7 +1247,8 @@ int run_dx(bgnn_ctx* ctx, int type, uint32_t m, uint32_t n, uint32_t k, const Ma
   g.out_type = type;
   g.out[0] = dx;
   g.ld_out = k;
-  return launch<EPI_LINEAR>(ctx, maps, g);
+  BGNN_TRY(make_chunk_maps(ctx, &maps, &g));
+  return launch<EPI_LINEAR>(ctx, maps, g, sh);
 }
 
 // dw_i = dz_i^T x: contraction over the m rows of both
@@ -821,15 +1262,19 @@ int run_dw(bgnn_ctx* ctx, int type, uint32_t m, uint32_t n, uint32_t k, const Ma
   g.in_type = type;
   g.a_mn = g.b_mn = 1;
   g.batches = (uint32_t)terms;
-  set_tile(&g, k <= 64 ? 64 : k <= 128 ? 128 : 256);
+  Shape sh = {k <= 64 ? 64u : k <= 128 ? 128u : 256u, 1};
+  if (sh.bn == 256 && n > BM) sh.cg = 2;
+  set_tile(&g, sh);
   g.nkb[0] = blocks_of(m, 64);
-  // ranges so that every SM has a tile, each of at least 8 k blocks
-  const uint64_t tiles = (uint64_t)blocks_of(n, BM) * blocks_of(k, g.bn) * terms;
-  uint64_t s = tiles >= (uint64_t)ctx->num_sms ? 1 : (uint64_t)ctx->num_sms / tiles;
+  // ranges so that every SM has a tile, each of at least 8 k blocks, and of at
+  // most MAX_PER: the tensor cores' own additions cost about 2^-24 a block
+  const uint64_t tiles = (uint64_t)blocks_of(n, BM * sh.cg) * blocks_of(k, g.bn) * terms;
+  uint64_t s = tiles * sh.cg >= (uint64_t)ctx->num_sms ? 1 : ctx->num_sms / (tiles * sh.cg);
   if (s > (g.nkb[0] + 7) / 8) s = (g.nkb[0] + 7) / 8;
   if (s < 1) s = 1;
   g.per = blocks_of(g.nkb[0], (uint32_t)s);
   if (g.per < 1) g.per = 1;
+  if (g.per > MAX_PER) g.per = MAX_PER;
   g.splits = blocks_of(g.nkb[0], g.per);
   if (g.splits < 1) g.splits = 1;
   if (m) {
@@ -841,14 +1286,26 @@ int run_dw(bgnn_ctx* ctx, int type, uint32_t m, uint32_t n, uint32_t k, const Ma
       BGNN_TRY(make_map(ctx, &maps.a[i], type, a, 64));
     }
   }
-  const uint64_t mn = (uint64_t)n * k;
-  BGNN_TRY(bgnn_tmp_alloc(ctx, part, mn * terms * g.splits * sizeof(float)));
-  g.part = part.as<float>();
-  g.out_type = BGNN_F32;
-  BGNN_TRY(launch<EPI_PARTIAL>(ctx, maps, g));
-  const uint64_t want = (mn * terms + 255) / 256, cap = (uint64_t)ctx->num_sms * 16;
+  g.out_type = type;
+  g.out[0] = dw[0];
+  g.out[1] = dw[1];
+  g.ld_out = k;
+  if (g.splits == 1) {
+    BGNN_TRY(make_chunk_maps(ctx, &maps, &g));
+    return launch<EPI_PARTIAL>(ctx, maps, g, sh);
+  }
+  // whole tiles of rows, so that a tile's last rows stay in its own part
+  g.part_rows = blocks_of(n, BM * sh.cg) * BM * sh.cg;
+  const uint32_t ldp = (k + 3) / 4 * 4;
+  const uint64_t prows = (uint64_t)g.part_rows * terms * g.splits;
+  BGNN_REQUIRE(ctx, prows < (1ull << 31), "weight gradient of %u x %u: too many parts", n, k);
+  BGNN_TRY(bgnn_tmp_alloc(ctx, part, prows * ldp * sizeof(float)));
+  g.tma_out = 1;
+  BGNN_TRY(make_chunk_map(ctx, &maps.out[0], BGNN_F32, {part.p, prows, k, ldp}));
+  BGNN_TRY(launch<EPI_PARTIAL>(ctx, maps, g, sh));
+  const uint64_t want = ((uint64_t)n * k * terms + 255) / 256, cap = (uint64_t)ctx->num_sms * 16;
   k_add_splits<<<(unsigned)(want < cap ? want : cap), 256, 0, ctx->stream>>>(
-      g.part, g.splits, (uint32_t)terms, mn, dw[0], dw[1], type);
+      part.as<float>(), g.splits, (uint32_t)terms, g.part_rows, ldp, n, k, dw[0], dw[1], type);
   BGNN_LAUNCHED(ctx);
   return BGNN_OK;
 }

@@ -44,10 +44,15 @@ def within(got, want, tol, what):
 
 
 def wide(x, how):
-    """x as a view with other strides: 'plain', 'rows' apart, or 'odd' (rows
-    that start off every vector)."""
+    """x as a view with other strides: 'plain', 'rows' apart, 'odd' (rows that
+    start off every vector) or 'vector' (rows that start on one, NaN behind)."""
     if how == "plain":
         return x
+    if how == "vector":
+        big = torch.full((x.shape[0], (x.shape[1] + 7) // 8 * 8 + 8), math.nan, dtype=x.dtype,
+                         device=x.device)
+        big[:, :x.shape[1]] = x
+        return big[:, :x.shape[1]]
     pad = 8 if how == "rows" else 3
     big = torch.full((x.shape[0], x.shape[1] + 2 * pad), math.nan, dtype=x.dtype, device=x.device)
     big[:, pad:-pad] = x
@@ -219,11 +224,9 @@ PRODUCTS = [  # m, k, n, type, act, bias, residual, out
 ]
 
 
-@pytest.mark.parametrize("how", ["plain", "rows", "odd"])
+@pytest.mark.parametrize("how", ["plain", "rows", "odd", "vector"])
 @pytest.mark.parametrize("m,k,n,t,act,tb,tr,to", PRODUCTS)
 def test_linear_fused(m, k, n, t, act, tb, tr, to, how):
-    if t == F8 and how == "odd":
-        how = "plain"  # NaN padding has no e4m3 fill
     g = gen(m + 3 * k + 5 * n)
     std = math.sqrt(2 / (k + n))
     x, xs, X = operand(g, m, k, t)
@@ -243,7 +246,7 @@ def test_linear_fused(m, k, n, t, act, tb, tr, to, how):
     assert got.dtype == to
 
 
-@pytest.mark.parametrize("how", ["plain", "odd"])
+@pytest.mark.parametrize("how", ["plain", "odd", "vector"])
 @pytest.mark.parametrize("m,k,n,t,act,tb", [
     (1, 1024, 512, BF, "silu", None), (1, 16, 16, F16, "gelu", F16), (130, 100, 47, BF, "silu", F32),
     (257, 256, 513, F16, "sigmoid", None), (40, 250, 33, BF, None, BF),
@@ -274,7 +277,7 @@ def test_gated_linear(m, k, n, t, act, tb, how):
     assert got.dtype == to
 
 
-@pytest.mark.parametrize("how", ["plain", "odd"])
+@pytest.mark.parametrize("how", ["plain", "odd", "vector"])
 @pytest.mark.parametrize("m,k,n,t,act,tb", [
     (1, 16, 16, BF, None, None), (1, 1024, 300, F16, "silu", F16), (5, 64, 47, BF, "gelu", BF),
     (130, 100, 256, F16, None, F32), (257, 256, 513, BF, "tanh", None),
@@ -319,7 +322,7 @@ def check_grads(t, X, W, dz, edz, gx, gw):
         assert g.dtype == t
 
 
-@pytest.mark.parametrize("how", ["plain", "odd"])
+@pytest.mark.parametrize("how", ["plain", "odd", "vector"])
 @pytest.mark.parametrize("m,k,n,t,act,tb", [
     (1, 64, 64, BF, "silu", None), (5, 100, 47, F16, "gelu", F16), (130, 256, 300, BF, "silu", F32),
     (2500, 128, 257, F16, "sigmoid", F16), (33, 1433, 24, BF, None, BF),
