@@ -176,15 +176,16 @@ __device__ __forceinline__ uint32_t peer_addr(uint32_t a, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
   return r;
 }
-// arrives on the issuing CTA's barrier
+// arrives on the issuing CTA's barrier.  It hands over tensor memory only, which
+// tcgen05.fence::before_thread_sync orders: no release of other memory.
 template <int CG>
 __device__ __forceinline__ void mbar_arrive_at(uint32_t a) {
   if constexpr (CG == 2)
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(
                      peer_addr(a, 0))
                  : "memory");
   else
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(a) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(a) : "memory");
 }
 // all threads of the CTA, or of the pair
 template <int CG>
@@ -327,26 +328,51 @@ __device__ __forceinline__ float rcp(float x) {
 constexpr float LOG2E = 1.4426950408889634f;
 // the logistic function 1 / (1 + 2^t), t = -x log2(e)
 __device__ __forceinline__ float sigmoid_t(float t) { return rcp(1.0f + ex2(t)); }
+// two f32 operations in one instruction
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"
+      " mul.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"
+      " add.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"
+      " mov.b64 w, {%6, %7};\n fma.rn.f32x2 z, x, y, w;\n mov.b64 {%0, %1}, z;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 // ... of two arguments with one reciprocal, 1/a = b/(ab): the epilogue's
 // exponentials and reciprocals share one unit of 16 lanes a clock.  t is held
 // at 63, so that ab stays finite; beyond, the value is 2^-63 instead of less,
 // which only ever enters as z * sigmoid (|z| > 43: 1e-17 of z).
-__device__ __forceinline__ float2 sigmoid_t2(float t0, float t1) {
-  const float a = 1.0f + ex2(fminf(t0, 63.0f)), b = 1.0f + ex2(fminf(t1, 63.0f));
-  const float r = rcp(a * b);
-  return make_float2(r * b, r * a);
+__device__ __forceinline__ float2 sigmoid_t2(float2 t) {
+  const float2 e = make_float2(ex2(fminf(t.x, 63.0f)), ex2(fminf(t.y, 63.0f)));
+  const float2 a = add2(e, both(1.0f));
+  return mul2(both(rcp(a.x * a.y)), make_float2(a.y, a.x));
 }
 constexpr float GELU_C = 0.7978845608028654f;  // sqrt(2/pi)
-// 0.5 (1 + tanh v) = sigmoid(2 v), v = sqrt(2/pi) (z + 0.044715 z^3), as t
-__device__ __forceinline__ float gelu_t(float z) {
-  constexpr float C = -2.0f * LOG2E * GELU_C;
-  return z * fmaf(C * 0.044715f, z * z, C);
-}
 template <int ACT>
 constexpr bool GATES = ACT == BGNN_ACT_SILU || ACT == BGNN_ACT_GELU;  // z sigmoid(..)
+// the gates' t: -z log2(e); gelu: 0.5 (1 + tanh v) = sigmoid(2 v),
+// v = sqrt(2/pi) (z + 0.044715 z^3)
 template <int ACT>
-__device__ __forceinline__ float gate_t(float z) {
-  return ACT == BGNN_ACT_SILU ? -LOG2E * z : gelu_t(z);
+__device__ __forceinline__ float2 gate_t2(float2 z) {
+  if constexpr (ACT == BGNN_ACT_SILU) return mul2(z, both(-LOG2E));
+  constexpr float C = -2.0f * LOG2E * GELU_C;
+  return mul2(z, fma2(mul2(z, z), both(C * 0.044715f), both(C)));
 }
 template <int ACT>
 __device__ __forceinline__ float act_one(float z, float p) {
@@ -360,15 +386,9 @@ __device__ __forceinline__ float act_one(float z, float p) {
 }
 // two activations
 template <int ACT>
-__device__ __forceinline__ void act_two(float& z0, float& z1, float p) {
-  if constexpr (GATES<ACT>) {
-    const float2 s = sigmoid_t2(gate_t<ACT>(z0), gate_t<ACT>(z1));
-    z0 *= s.x;
-    z1 *= s.y;
-  } else {
-    z0 = act_one<ACT>(z0, p);
-    z1 = act_one<ACT>(z1, p);
-  }
+__device__ __forceinline__ float2 act_two(float2 z, float p) {
+  if constexpr (GATES<ACT>) return mul2(z, sigmoid_t2(gate_t2<ACT>(z)));
+  return make_float2(act_one<ACT>(z.x, p), act_one<ACT>(z.y, p));
 }
 // act(z) and act'(z); s: sigmoid(..) of the gates
 template <int ACT>
@@ -401,11 +421,11 @@ __device__ __forceinline__ float2 act_grad(float z, float s, float p) {
   return make_float2(z, 1.0f);
 }
 template <int ACT>
-__device__ __forceinline__ void act_grad_two(float z0, float z1, float p, float2& f0, float2& f1) {
+__device__ __forceinline__ void act_grad_two(float2 z, float p, float2& f0, float2& f1) {
   float2 s = make_float2(0.0f, 0.0f);
-  if constexpr (GATES<ACT>) s = sigmoid_t2(gate_t<ACT>(z0), gate_t<ACT>(z1));
-  f0 = act_grad<ACT>(z0, s.x, p);
-  f1 = act_grad<ACT>(z1, s.y, p);
+  if constexpr (GATES<ACT>) s = sigmoid_t2(gate_t2<ACT>(z));
+  f0 = act_grad<ACT>(z.x, s.x, p);
+  f1 = act_grad<ACT>(z.y, s.y, p);
 }
 // Runs f(Act<..>) for an activation known at run time.  One branch a chunk of
 // 32 elements: the switch inside the element loop made the code of every
@@ -555,15 +575,20 @@ struct Tile {
   uint32_t m0, n0, batch, split;
 };
 template <int EPI, int CG>
-__device__ __forceinline__ Tile tile_at(const GemmArgs& g, uint64_t t, uint32_t n_tiles,
+__device__ __forceinline__ Tile tile_at(const GemmArgs& g, uint32_t t, uint32_t n_tiles,
                                         uint32_t m_tiles, uint32_t wn) {
   Tile r;
-  const uint64_t q = t / n_tiles;
-  r.n0 = (uint32_t)(t % n_tiles) * wn;
-  r.m0 = (uint32_t)(q % m_tiles) * (BM * CG);
-  const uint32_t z = (uint32_t)(q / m_tiles);
-  r.batch = EPI == EPI_PARTIAL ? z % g.batches : 0;
-  r.split = EPI == EPI_PARTIAL ? z / g.batches : 0;
+  const uint32_t q = t / n_tiles;
+  r.n0 = (t - q * n_tiles) * wn;
+  if (EPI == EPI_PARTIAL) {
+    const uint32_t z = q / m_tiles;
+    r.m0 = (q - z * m_tiles) * (BM * CG);
+    r.split = z / g.batches;
+    r.batch = z - r.split * g.batches;
+  } else {
+    r.m0 = q * (BM * CG);
+    r.split = r.batch = 0;
+  }
   return r;
 }
 
@@ -611,9 +636,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t wn = TWO ? g.bn / 2 : g.bn;  // output columns of a tile
   const uint32_t bl = g.bn / CG;              // rows of the B tile that this CTA loads
   const uint32_t n_tiles = (g.n + wn - 1) / wn, m_tiles = (g.m + BM * CG - 1) / (BM * CG);
-  const uint64_t tiles = (uint64_t)m_tiles * n_tiles *
-                         (EPI == EPI_PARTIAL ? (uint64_t)g.batches * g.splits : 1ull);
-  const uint64_t t_first = blockIdx.x / CG, t_step = gridDim.x / CG;
+  const uint32_t tiles = m_tiles * n_tiles * (EPI == EPI_PARTIAL ? g.batches * g.splits : 1u);
+  const uint32_t t_first = blockIdx.x / CG, t_step = gridDim.x / CG;
   const uint32_t nkb = g.nkb[0] + g.nkb[1];
   // k blocks [first, last) of a tile
   auto kb_first = [&](const Tile& t) { return EPI == EPI_PARTIAL ? t.split * g.per : 0u; };
@@ -630,7 +654,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       uint64_t filled = 0;
       const uint32_t tx = CG * (A_BYTES + bl * 128);
       const int kw = g.fp8 ? 128 : 64;  // elements of a k block
-      for (uint64_t t = t_first; t < tiles; t += t_step) {
+      for (uint32_t t = t_first; t < tiles; t += t_step) {
         const Tile ti = tile_at<EPI, CG>(g, t, n_tiles, m_tiles, wn);
         const int am = (int)(ti.m0 + rank * BM);
         const uint32_t e = kb_last(ti);
@@ -677,7 +701,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (lane == 0 && rank == 0) {
       uint32_t s = 0, ph = 0, buf = 0, aph = 0;
       const uint32_t step_a = g.a_mn ? 2048u : 32u, step_b = g.b_mn ? 2048u : 32u;
-      for (uint64_t t = t_first; t < tiles; t += t_step) {
+      for (uint32_t t = t_first; t < tiles; t += t_step) {
         const Tile ti = tile_at<EPI, CG>(g, t, n_tiles, m_tiles, wn);
         const uint32_t last = kb_last(ti);
         uint32_t kb = kb_first(ti);
@@ -731,7 +755,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (++buf == 2) buf = 0, aph ^= 1u;
     };
     bool gave_up = false;
-    for (uint64_t t = t_first; t < tiles && !gave_up; t += t_step) {
+    for (uint32_t t = t_first; t < tiles && !gave_up; t += t_step) {
       const Tile ti = tile_at<EPI, CG>(g, t, n_tiles, m_tiles, wn);
       const uint32_t k_first = kb_first(ti), k_last = kb_last(ti);
       const bool any_k = k_first < k_last;
@@ -825,8 +849,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (g.act != BGNN_ACT_NONE)
           with_act(g.act, [&](auto act) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 2)
-              act_two<decltype(act)::value>(v[j], v[j + 1], g.act_p);
+            for (int j = 0; j < 32; j += 2) {
+              const float2 f = act_two<decltype(act)::value>(make_float2(v[j], v[j + 1]), g.act_p);
+              v[j] = f.x;
+              v[j + 1] = f.y;
+            }
           });
         if (g.other) take(col0, next, [&](int j, float o) { v[j] += o; });
         give(v, col0, 0, g.out_type, row0);
@@ -903,7 +930,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
               for (int j = 0; j < 32; j += 2) {
                 float2 f0, f1;
-                act_grad_two<decltype(act)::value>(v[j], v[j + 1], g.act_p, f0, f1);
+                act_grad_two<decltype(act)::value>(make_float2(v[j], v[j + 1]), g.act_p, f0, f1);
                 v[j] = o[j] * f0.y;
                 v[j + 1] = o[j + 1] * f1.y;
               }
@@ -915,9 +942,11 @@ __global__ void __launch_bounds__(THREADS, 1)
             with_act(g.act, [&](auto act) {
 #pragma unroll
               for (int j = 0; j < 32; j += 2) {
-                act_two<decltype(act)::value>(v[j], v[j + 1], g.act_p);
-                v[j] *= u[j];
-                v[j + 1] *= u[j + 1];
+                const float2 f =
+                    mul2(act_two<decltype(act)::value>(make_float2(v[j], v[j + 1]), g.act_p),
+                         make_float2(u[j], u[j + 1]));
+                v[j] = f.x;
+                v[j + 1] = f.y;
               }
             });
             give(v, col0, 0, g.out_type, row0);
@@ -930,7 +959,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
               for (int j = 0; j < 32; j += 2) {
                 float2 f0, f1;
-                act_grad_two<decltype(act)::value>(v[j], v[j + 1], g.act_p, f0, f1);
+                act_grad_two<decltype(act)::value>(make_float2(v[j], v[j + 1]), g.act_p, f0, f1);
                 v[j] = o[j] * u[j] * f0.y;  // dg
                 v[j + 1] = o[j + 1] * u[j + 1] * f1.y;
                 u[j] = o[j] * f0.x;  // du
@@ -1193,6 +1222,7 @@ int launch(bgnn_ctx* ctx, const Maps& maps, GemmArgs& g, const Shape& s) {
   const uint32_t wn = TWO ? s.bn / 2 : s.bn;
   const uint64_t tiles = (uint64_t)blocks_of(g.m, BM * s.cg) * blocks_of(g.n, wn) *
                          (EPI == EPI_PARTIAL ? (uint64_t)g.batches * g.splits : 1ull);
+  BGNN_REQUIRE(ctx, tiles < (1ull << 31), "product of %u x %u: too many tiles", g.m, g.n);
   return s.cg == 2 ? launch_cg<EPI, 2>(ctx, maps, g, tiles) : launch_cg<EPI, 1>(ctx, maps, g, tiles);
 }
 
