@@ -57,7 +57,7 @@ constexpr int RING_BYTES = 160 * 1024;
 constexpr int SMEM_BYTES = 1024 + RING_BYTES + EPI_WARPS * WARP_BYTES + 512;
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory of one SM");
 constexpr uint32_t SPIN_LIMIT = 1u << 24;     // polls before a wait gives up,
-constexpr uint64_t SPIN_NS = 2000000000ull;  // or this long
+constexpr long long SPIN_CLOCKS = 4000000000ll;  // or clocks (about two seconds)
 
 enum Epi : int { EPI_LINEAR, EPI_LINEAR_F32, EPI_GATED, EPI_LINEAR_BWD, EPI_GATED_BWD, EPI_PARTIAL };
 // k blocks whose products one accumulator takes before they are added in f32
@@ -123,20 +123,17 @@ __device__ __forceinline__ bool mbar_try(uint32_t a, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ uint64_t now_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-  return t;
-}
 // bounded wait; false when it gave up or another role already did
 __device__ __forceinline__ bool mbar_wait(uint32_t a, uint32_t parity, volatile uint32_t* abort_flag,
                                           int* err, int where) {
-  if (mbar_try(a, parity)) return true;
-  const uint64_t t0 = now_ns();
+  long long t0 = 0;
   for (uint32_t i = 0; i < SPIN_LIMIT; i++) {
     if (mbar_try(a, parity)) return true;
-    if (*abort_flag) return false;
-    if ((i & 63u) == 63u && now_ns() - t0 > SPIN_NS) break;
+    if ((i & 31u) == 31u) {
+      if (*abort_flag) return false;
+      if (t0 == 0) t0 = clock64();
+      else if (clock64() - t0 > SPIN_CLOCKS) break;
+    }
   }
   *abort_flag = 1u;
   dev_raise(err, DEVERR_TIMEOUT, (uint64_t)blockIdx.x, where);
@@ -144,9 +141,9 @@ __device__ __forceinline__ bool mbar_wait(uint32_t a, uint32_t parity, volatile 
 }
 // for what is in flight when a role has given up
 __device__ __forceinline__ void mbar_drain(uint32_t a, uint32_t parity) {
-  const uint64_t t0 = now_ns();
+  const long long t0 = clock64();
   for (uint32_t i = 0; i < SPIN_LIMIT; i++)
-    if (mbar_try(a, parity) || now_ns() - t0 > SPIN_NS / 4) return;
+    if (mbar_try(a, parity) || clock64() - t0 > SPIN_CLOCKS / 4) return;
 }
 // CG: CTAs that share one product (cta_group), 1 or a pair
 template <int CG>
@@ -650,45 +647,51 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == EPI_WARPS) {
     // ---- TMA producer ----
     if (lane == 0) {
-      uint32_t s = 0, ph = 0;
+      uint32_t s = 0, ph = 0, st = base;
       uint64_t filled = 0;
       const uint32_t tx = CG * (A_BYTES + bl * 128);
       const int kw = g.fp8 ? 128 : 64;  // elements of a k block
+      // both CTAs' loads count on the issuing CTA's barriers
+      const uint32_t b_land = CG == 2 ? peer_addr(b_full, 0) : b_full;
+      const bool a_mn = g.a_mn, b_mn = g.b_mn;
+      const uint32_t nkb0 = g.nkb[0], stage_bytes = g.stage_bytes;
       for (uint32_t t = t_first; t < tiles; t += t_step) {
         const Tile ti = tile_at<EPI, CG>(g, t, n_tiles, m_tiles, wn);
         const int am = (int)(ti.m0 + rank * BM);
+        const int bn0 = (int)(TWO ? ti.n0 : ti.n0 + rank * bl);
         const uint32_t e = kb_last(ti);
-        for (uint32_t kb = kb_first(ti); kb < e; kb++) {
+        uint32_t kb = kb_first(ti);
+        // dw: the batch's A; else the segment's A and B
+        const CUtensorMap* ma = &maps.a[EPI == EPI_PARTIAL ? ti.batch : 0];
+        const CUtensorMap* mb = &maps.b[TWO && CG == 2 ? rank : 0];  // a weight a CTA
+        int k0 = (int)kb * kw;
+        for (; kb < e; kb++, k0 += kw) {
+          if (EPI != EPI_PARTIAL && !TWO && kb == nkb0) {  // the second segment
+            ma = &maps.a[1];
+            mb = &maps.b[1];
+            k0 = 0;
+          }
           if (!mbar_wait(b_empty + 8 * s, ph ^ 1u, abort_flag, g.err, 70)) goto drain;
           if (rank == 0) mbar_expect_tx(b_full + 8 * s, tx);
-          const int seg = EPI == EPI_PARTIAL ? (int)ti.batch : (kb >= g.nkb[0] ? 1 : 0);
-          const int k0 = (int)((EPI != EPI_PARTIAL && seg ? kb - g.nkb[0] : kb)) * kw;
-          const uint32_t st = base + s * g.stage_bytes;
-          // both CTAs' loads count on the issuing CTA's barrier
-          const uint32_t bar = CG == 2 ? peer_addr(b_full + 8 * s, 0) : b_full + 8 * s;
-          if (g.a_mn) {
+          const uint32_t bar = b_land + 8 * s;
+          if (a_mn) {
+#pragma unroll
             for (int i = 0; i < BM / 64; i++)
-              tma_load_2d<CG>(st + i * 8192, &maps.a[seg], am + i * 64, k0, bar);
+              tma_load_2d<CG>(st + i * 8192, ma, am + i * 64, k0, bar);
           } else {
-            tma_load_2d<CG>(st, &maps.a[seg], k0, am, bar);
+            tma_load_2d<CG>(st, ma, k0, am, bar);
           }
-          if (TWO && CG == 2) {  // one weight a CTA
-            tma_load_2d<CG>(st + A_BYTES, &maps.b[rank], k0, (int)ti.n0, bar);
-          } else if (TWO) {
-            tma_load_2d<CG>(st + A_BYTES, &maps.b[0], k0, (int)ti.n0, bar);
-            tma_load_2d<CG>(st + A_BYTES + wn * 128, &maps.b[1], k0, (int)ti.n0, bar);
+          if (b_mn) {
+            for (uint32_t i = 0; i < bl; i += 64)
+              tma_load_2d<CG>(st + A_BYTES + i * 128, mb, bn0 + (int)i, k0, bar);
           } else {
-            const CUtensorMap* mb = EPI == EPI_PARTIAL ? &maps.b[0] : &maps.b[seg];
-            const int bn0 = (int)(ti.n0 + rank * bl);
-            if (g.b_mn) {
-              for (uint32_t i = 0; i < bl / 64; i++)
-                tma_load_2d<CG>(st + A_BYTES + i * 8192, mb, bn0 + (int)i * 64, k0, bar);
-            } else {
-              tma_load_2d<CG>(st + A_BYTES, mb, k0, bn0, bar);
-            }
+            tma_load_2d<CG>(st + A_BYTES, mb, k0, bn0, bar);
+            if (TWO && CG == 1)
+              tma_load_2d<CG>(st + A_BYTES + wn * 128, &maps.b[1], k0, bn0, bar);
           }
           filled++;
-          if (++s == S) s = 0, ph ^= 1u;
+          st += stage_bytes;
+          if (++s == S) s = 0, ph ^= 1u, st = base;
         }
       }
     drain:
@@ -700,37 +703,43 @@ __global__ void __launch_bounds__(THREADS, 1)
     // ---- MMA issuer ----
     if (lane == 0 && rank == 0) {
       uint32_t s = 0, ph = 0, buf = 0, aph = 0;
-      const uint32_t step_a = g.a_mn ? 2048u : 32u, step_b = g.b_mn ? 2048u : 32u;
-      for (uint32_t t = t_first; t < tiles; t += t_step) {
-        const Tile ti = tile_at<EPI, CG>(g, t, n_tiles, m_tiles, wn);
-        const uint32_t last = kb_last(ti);
-        uint32_t kb = kb_first(ti);
-        do {  // a piece of the contraction into one accumulator
-          const uint32_t e = EPI == EPI_LINEAR_F32 && last - kb > PIECE ? kb + PIECE : last;
-          if (!mbar_wait(b_acce + 8 * buf, aph ^ 1u, abort_flag, g.err, 71)) goto stop;
-          tc_fence_after();
-          const uint32_t d = tmem + buf * g.bn;
-          uint32_t acc = 0u;
-          for (; kb < e; kb++) {
-            if (!mbar_wait(b_full + 8 * s, ph, abort_flag, g.err, 72)) goto stop;
+      // The issuing thread's own instructions bound a stage once (about 1000
+      // clocks against 512 of products): the descriptors are one addition each.
+      const uint64_t desc_a = smem_desc(base, g.a_mn), desc_b = smem_desc(base + A_BYTES, g.b_mn);
+      const uint32_t step_a = (g.a_mn ? 2048u : 32u) >> 4, step_b = (g.b_mn ? 2048u : 32u) >> 4;
+      const uint32_t stage16 = g.stage_bytes >> 4, idesc = g.idesc, bn = g.bn;
+      auto issue = [&](auto fp8) -> bool {
+        for (uint32_t t = t_first; t < tiles; t += t_step) {
+          const Tile ti = tile_at<EPI, CG>(g, t, n_tiles, m_tiles, wn);
+          const uint32_t last = kb_last(ti);
+          uint32_t kb = kb_first(ti);
+          do {  // a piece of the contraction into one accumulator
+            const uint32_t e = EPI == EPI_LINEAR_F32 && last - kb > PIECE ? kb + PIECE : last;
+            if (!mbar_wait(b_acce + 8 * buf, aph ^ 1u, abort_flag, g.err, 71)) return false;
             tc_fence_after();
-            const uint32_t st = base + s * g.stage_bytes;
+            const uint32_t d = tmem + buf * bn;
+            uint32_t acc = 0u;
+            for (; kb < e; kb++) {
+              if (!mbar_wait(b_full + 8 * s, ph, abort_flag, g.err, 72)) return false;
+              tc_fence_after();
+              const uint64_t da = desc_a + s * stage16, db = desc_b + s * stage16;
 #pragma unroll
-            for (uint32_t kk = 0; kk < 4; kk++) {
-              const uint64_t da = smem_desc(st + kk * step_a, g.a_mn);
-              const uint64_t db = smem_desc(st + A_BYTES + kk * step_b, g.b_mn);
-              if (g.fp8) mma_f8<CG>(d, da, db, g.idesc, acc);
-              else mma_f16<CG>(d, da, db, g.idesc, acc);
-              acc = 1u;
+              for (uint32_t kk = 0; kk < 4; kk++) {
+                if (decltype(fp8)::value) mma_f8<CG>(d, da + kk * step_a, db + kk * step_b, idesc, acc);
+                else mma_f16<CG>(d, da + kk * step_a, db + kk * step_b, idesc, acc);
+                acc = 1u;
+              }
+              mma_commit<CG>(b_empty + 8 * s);
+              if (++s == S) s = 0, ph ^= 1u;
             }
-            mma_commit<CG>(b_empty + 8 * s);
-            if (++s == S) s = 0, ph ^= 1u;
-          }
-          mma_commit<CG>(b_accf + 8 * buf);
-          if (++buf == 2) buf = 0, aph ^= 1u;
-        } while (kb < last);
-      }
-    stop:
+            mma_commit<CG>(b_accf + 8 * buf);
+            if (++buf == 2) buf = 0, aph ^= 1u;
+          } while (kb < last);
+        }
+        return true;
+      };
+      if (g.fp8) issue(std::true_type{});
+      else issue(std::false_type{});
       // every product issued is done before tensor memory is freed
       mma_commit_here<CG>(b_last);
       mbar_drain(b_last, 0);
