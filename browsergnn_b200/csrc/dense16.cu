@@ -16,14 +16,17 @@
 // the two products that follow take it as an operand.
 //
 // Kernel: persistent, one CTA an SM, 128 x BN output tiles, warp-specialised:
-//   warp 8    TMA producer: per k block (128 bytes of k) the A tile and the B
+//   warp 16   TMA producer: per k block (128 bytes of k) the A tile and the B
 //             tile into a ring of shared-memory stages, 128-byte swizzle;
-//   warp 9    MMA issuer (one thread): tcgen05.mma, M = 128, N = BN, into one
+//   warp 17   MMA issuer (one thread): tcgen05.mma, M = 128, N = BN, into one
 //             of two tensor-memory accumulators;
-//   warps 0-7 epilogue: warp w takes the accumulator lanes (rows) of its
-//             quadrant w % 4 and every other 32-column chunk, and turns them
-//             round through shared memory so that global reads and writes
-//             run along rows.
+//   warps 0-15 epilogue: warp w takes the accumulator lanes (rows) of its
+//             quadrant w % 4 and every fourth 32-column chunk; chunks come in
+//             and go out by TMA through two shared-memory slots a warp, or,
+//             where TMA cannot take the rows, turned round there and read and
+//             written along rows.  Sixteen warps, four a scheduler: with eight
+//             the activations of a short contraction ran at a third of the
+//             issue rate and bound the kernel.
 // An operand whose contraction runs down its rows (w in dx, both in dw) is
 // read as it lies ("MN-major": boxes of 64 columns x 64 rows), never
 // transposed in memory.  The gated kernels load BN/2 rows of each weight side
@@ -47,12 +50,15 @@
 namespace {
 
 constexpr int BM = 128;
-constexpr int EPI_WARPS = 8;
-constexpr int THREADS = (EPI_WARPS + 2) * 32;
+constexpr int EPI_WARPS = 16;
+constexpr int THREADS = (EPI_WARPS + 4) * 32;  // five warpgroups; warps 18 and 19 idle
+// Registers a thread: at most 96 at launch (65,536 / 640), then split unevenly:
+// 4 * 104 + 64 = 5 * 96.
+constexpr int EPI_REGS = 104, ISSUE_REGS = 64;
 constexpr int MAX_STAGES = 8;
 constexpr int A_BYTES = BM * 128;
-constexpr int SLOT_BYTES = 32 * 32 * 4;     // a 32 x 32 chunk in f32
-constexpr int WARP_BYTES = 2 * SLOT_BYTES;  // an epilogue warp's chunk in and chunk out
+constexpr int SLOT_BYTES = 32 * 64;         // 32 rows x 32 16-bit or 16 f32 columns
+constexpr int WARP_BYTES = 2 * SLOT_BYTES;  // an epilogue warp's two slots
 constexpr int RING_BYTES = 160 * 1024;
 constexpr int SMEM_BYTES = 1024 + RING_BYTES + EPI_WARPS * WARP_BYTES + 512;
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory of one SM");
@@ -67,7 +73,7 @@ constexpr uint32_t MAX_PER = 512;  // k blocks of a dw range
 
 // One contraction segment: A [m, k] and B [n, k] tiles of one or two tensors.
 // Where `b1` is used (gated), B's tile is rows of b0 above rows of b1.
-// in / out: the residual or upstream gradient and the outputs in 32 x 32 boxes,
+// in / out: the residual or upstream gradient and the outputs in boxes of a slot,
 // where TMA can take them.
 struct Maps {
   CUtensorMap a[2], b[2], in, out[2];
@@ -351,14 +357,12 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return r;
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
-// ... of two arguments with one reciprocal, 1/a = b/(ab): the epilogue's
-// exponentials and reciprocals share one unit of 16 lanes a clock.  t is held
-// at 63, so that ab stays finite; beyond, the value is 2^-63 instead of less,
-// which only ever enters as z * sigmoid (|z| > 43: 1e-17 of z).
+// ... of two arguments.  (One reciprocal for both, 1/a = b/(ab), saves a
+// quarter of the special-function work but costs three more instructions a
+// pair and a clamp; the epilogue is bound by instructions, not by that unit.)
 __device__ __forceinline__ float2 sigmoid_t2(float2 t) {
-  const float2 e = make_float2(ex2(fminf(t.x, 63.0f)), ex2(fminf(t.y, 63.0f)));
-  const float2 a = add2(e, both(1.0f));
-  return mul2(both(rcp(a.x * a.y)), make_float2(a.y, a.x));
+  const float2 a = add2(make_float2(ex2(t.x), ex2(t.y)), both(1.0f));
+  return make_float2(rcp(a.x), rcp(a.y));
 }
 constexpr float GELU_C = 0.7978845608028654f;  // sqrt(2/pi)
 template <int ACT>
@@ -393,9 +397,9 @@ __device__ __forceinline__ float2 act_grad(float z, float s, float p) {
   if constexpr (ACT == BGNN_ACT_SILU) return make_float2(z * s, s * fmaf(z, 1.0f - s, 1.0f));
   if constexpr (ACT == BGNN_ACT_GELU) {
     const float dv = 2.0f * GELU_C * fmaf(3.0f * 0.044715f * z, z, 1.0f);
-    // far out s (1 - s) is 0, or z s is 2^-63 z; dv must not make a NaN of it
+    // far out s (1 - s) is 0; dv must not make a NaN of it
     const float q = s * (1.0f - s);
-    return make_float2(z * s, q < 1e-18f ? s : fmaf(z * q, dv, s));
+    return make_float2(z * s, q == 0.0f ? s : fmaf(z * q, dv, s));
   }
   if constexpr (ACT == BGNN_ACT_RELU)
     return z > 0.0f ? make_float2(z, 1.0f) : make_float2(0.0f, 0.0f);
@@ -444,13 +448,9 @@ __device__ __forceinline__ void with_act(int act, F&& f) {
   }
 }
 
-// ---- chunk slots: 32 rows of 128 bytes (f32) or 64 bytes (16 bits), 16-byte
-// units swizzled as TMA does, so that a row a lane has no bank conflicts ---------
-__device__ __forceinline__ float4* turn_unit(void* slot, int row, int unit) {
-  return reinterpret_cast<float4*>(static_cast<char*>(slot) + row * 128 +
-                                   ((unit ^ (row & 7)) << 4));
-}
-__device__ __forceinline__ uint4* turn_unit16(void* slot, int row, int unit) {
+// ---- slots: 32 rows of 64 bytes, 16-byte units swizzled as TMA's 64-byte mode
+// does, so that a row a lane has no bank conflicts ------------------------------
+__device__ __forceinline__ uint4* slot_unit(void* slot, int row, int unit) {
   return reinterpret_cast<uint4*>(static_cast<char*>(slot) + row * 64 +
                                   ((unit ^ ((row >> 1) & 3)) << 4));
 }
@@ -458,49 +458,30 @@ template <int DT>
 __device__ __forceinline__ void put_row16(void* slot, int row, const float (&v)[32]) {
 #pragma unroll
   for (int u = 0; u < 4; u++)
-    *turn_unit16(slot, row, u) =
+    *slot_unit(slot, row, u) =
         make_uint4(pack2<DT>(v[8 * u], v[8 * u + 1]), pack2<DT>(v[8 * u + 2], v[8 * u + 3]),
                    pack2<DT>(v[8 * u + 4], v[8 * u + 5]), pack2<DT>(v[8 * u + 6], v[8 * u + 7]));
 }
-// a row of a chunk into a slot, rounded to the element type
-__device__ __forceinline__ void put_row(void* slot, int row, int dt, const float (&v)[32]) {
-  if (dt == BGNN_F32) {
+// eight 16-bit elements of a slot's unit
+__device__ __forceinline__ void unit16(const uint4 q, int dt, float (&o)[8]) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-    for (int u = 0; u < 8; u++)
-      *turn_unit(slot, row, u) = make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
-  } else if (dt == BGNN_BF16) {
-    put_row16<BGNN_BF16>(slot, row, v);
-  } else {
-    put_row16<BGNN_F16>(slot, row, v);
+  for (int i = 0; i < 4; i++) {
+    if (dt == BGNN_BF16) {
+      o[2 * i] = __uint_as_float(w[i] << 16);
+      o[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      o[2 * i] = f.x;
+      o[2 * i + 1] = f.y;
+    }
   }
 }
-// a row of a slot: f(i, value) for its 32 elements
-template <class F>
-__device__ __forceinline__ void each_of_row(void* slot, int row, int dt, F&& f) {
-  if (dt == BGNN_F32) {
-#pragma unroll
-    for (int u = 0; u < 8; u++) {
-      const float4 w = *turn_unit(slot, row, u);
-      f(4 * u, w.x), f(4 * u + 1, w.y), f(4 * u + 2, w.z), f(4 * u + 3, w.w);
-    }
-  } else {
-#pragma unroll
-    for (int u = 0; u < 4; u++) {
-      const uint4 q = *turn_unit16(slot, row, u);
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        if (dt == BGNN_BF16) {
-          f(8 * u + 2 * i, __uint_as_float(w[i] << 16));
-          f(8 * u + 2 * i + 1, __uint_as_float(w[i] & 0xffff0000u));
-        } else {
-          const float2 q2 = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-          f(8 * u + 2 * i, q2.x);
-          f(8 * u + 2 * i + 1, q2.y);
-        }
-      }
-    }
-  }
+// both slots as 32 rows x 32 f32: where rows cannot go by TMA and are turned
+// round by the warp
+__device__ __forceinline__ float4* turn_unit(void* slots, int row, int unit) {
+  return reinterpret_cast<float4*>(static_cast<char*>(slots) + row * 128 +
+                                   ((unit ^ (row & 7)) << 4));
 }
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, uint32_t src) {
   asm volatile(
@@ -567,27 +548,47 @@ __device__ __forceinline__ bool vec4_ok(const void* p, int dt, uint64_t ld) {
   return ((uintptr_t)p & (b - 1)) == 0 && ld % 4 == 0;
 }
 
-// what a tile index stands for
+// the tiles of a CTA (pair), columns fastest
 struct Tile {
   uint32_t m0, n0, batch, split;
 };
 template <int EPI, int CG>
-__device__ __forceinline__ Tile tile_at(const GemmArgs& g, uint32_t t, uint32_t n_tiles,
-                                        uint32_t m_tiles, uint32_t wn) {
-  Tile r;
-  const uint32_t q = t / n_tiles;
-  r.n0 = (t - q * n_tiles) * wn;
-  if (EPI == EPI_PARTIAL) {
-    const uint32_t z = q / m_tiles;
-    r.m0 = (q - z * m_tiles) * (BM * CG);
-    r.split = z / g.batches;
-    r.batch = z - r.split * g.batches;
-  } else {
-    r.m0 = q * (BM * CG);
-    r.split = r.batch = 0;
+struct Tiles {
+  const GemmArgs& g;
+  uint32_t n_tiles, m_tiles, wn, left, q, nt, step_q, step_n;
+  __device__ __forceinline__ Tiles(const GemmArgs& args, uint32_t width) : g(args), wn(width) {
+    n_tiles = (g.n + wn - 1) / wn;
+    m_tiles = (g.m + BM * CG - 1) / (BM * CG);
+    const uint32_t tiles = m_tiles * n_tiles * (EPI == EPI_PARTIAL ? g.batches * g.splits : 1u);
+    const uint32_t first = blockIdx.x / CG, step = gridDim.x / CG;
+    left = (tiles - first + step - 1) / step;  // the grid has at most `tiles` CTAs (pairs)
+    q = first / n_tiles;
+    nt = first - q * n_tiles;
+    step_q = step / n_tiles;
+    step_n = step - step_q * n_tiles;
   }
-  return r;
-}
+  __device__ __forceinline__ bool more() const { return left != 0; }
+  __device__ __forceinline__ void next() {
+    left--;
+    q += step_q;
+    nt += step_n;
+    if (nt >= n_tiles) nt -= n_tiles, q++;
+  }
+  __device__ __forceinline__ Tile at() const {
+    Tile r;
+    r.n0 = nt * wn;
+    if (EPI == EPI_PARTIAL) {
+      const uint32_t z = q / m_tiles;
+      r.m0 = (q - z * m_tiles) * (BM * CG);
+      r.split = z / g.batches;
+      r.batch = z - r.split * g.batches;
+    } else {
+      r.m0 = q * (BM * CG);
+      r.split = r.batch = 0;
+    }
+    return r;
+  }
+};
 
 template <int EPI, int CG>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -632,9 +633,6 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   const uint32_t wn = TWO ? g.bn / 2 : g.bn;  // output columns of a tile
   const uint32_t bl = g.bn / CG;              // rows of the B tile that this CTA loads
-  const uint32_t n_tiles = (g.n + wn - 1) / wn, m_tiles = (g.m + BM * CG - 1) / (BM * CG);
-  const uint32_t tiles = m_tiles * n_tiles * (EPI == EPI_PARTIAL ? g.batches * g.splits : 1u);
-  const uint32_t t_first = blockIdx.x / CG, t_step = gridDim.x / CG;
   const uint32_t nkb = g.nkb[0] + g.nkb[1];
   // k blocks [first, last) of a tile
   auto kb_first = [&](const Tile& t) { return EPI == EPI_PARTIAL ? t.split * g.per : 0u; };
@@ -644,6 +642,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     return e < nkb ? e : nkb;
   };
 
+  if (warp >= EPI_WARPS) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(ISSUE_REGS));
   if (warp == EPI_WARPS) {
     // ---- TMA producer ----
     if (lane == 0) {
@@ -655,8 +655,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint32_t b_land = CG == 2 ? peer_addr(b_full, 0) : b_full;
       const bool a_mn = g.a_mn, b_mn = g.b_mn;
       const uint32_t nkb0 = g.nkb[0], stage_bytes = g.stage_bytes;
-      for (uint32_t t = t_first; t < tiles; t += t_step) {
-        const Tile ti = tile_at<EPI, CG>(g, t, n_tiles, m_tiles, wn);
+      for (Tiles<EPI, CG> ts(g, wn); ts.more(); ts.next()) {
+        const Tile ti = ts.at();
         const int am = (int)(ti.m0 + rank * BM);
         const int bn0 = (int)(TWO ? ti.n0 : ti.n0 + rank * bl);
         const uint32_t e = kb_last(ti);
@@ -709,8 +709,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint32_t step_a = (g.a_mn ? 2048u : 32u) >> 4, step_b = (g.b_mn ? 2048u : 32u) >> 4;
       const uint32_t stage16 = g.stage_bytes >> 4, idesc = g.idesc, bn = g.bn;
       auto issue = [&](auto fp8) -> bool {
-        for (uint32_t t = t_first; t < tiles; t += t_step) {
-          const Tile ti = tile_at<EPI, CG>(g, t, n_tiles, m_tiles, wn);
+        for (Tiles<EPI, CG> ts(g, wn); ts.more(); ts.next()) {
+          const Tile ti = ts.at();
           const uint32_t last = kb_last(ti);
           uint32_t kb = kb_first(ti);
           do {  // a piece of the contraction into one accumulator
@@ -744,18 +744,18 @@ __global__ void __launch_bounds__(THREADS, 1)
       mma_commit_here<CG>(b_last);
       mbar_drain(b_last, 0);
     }
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(EPI_REGS));
     // ---- epilogue ----
-    const int quad = warp & 3, half = warp >> 2;
-    uint8_t* in_slot = gbase + RING_BYTES + warp * WARP_BYTES;
-    uint8_t* out_slot = in_slot + SLOT_BYTES;  // one f32 chunk, or two 16-bit ones in turn
+    const int quad = warp & 3, group = warp >> 2;  // rows; every fourth 32-column chunk
+    uint8_t* slots = gbase + RING_BYTES + warp * WARP_BYTES;
     const uint32_t in_bar = b_in + 8 * warp;
-    uint32_t buf = 0, aph = 0, in_ph = 0, out_at = 0;
+    uint32_t buf = 0, aph = 0, in_ph = 0, out_at = 1;
     const bool parts = EPI == EPI_PARTIAL && g.part_rows;
     const bool vec_out = vec4_ok(g.out[0], g.out_type, g.ld_out) &&
                          (!g.out[1] || vec4_ok(g.out[1], g.out_type, g.ld_out));
     const bool vec_other = g.other && vec4_ok(g.other, g.other_type, g.ld_other);
-    const uint32_t in_bytes = g.other_type == BGNN_F32 ? 4096u : 2048u;
     // hands the accumulator back once every lane has read it
     auto release = [&]() {
       tc_fence_before();
@@ -764,70 +764,116 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (++buf == 2) buf = 0, aph ^= 1u;
     };
     bool gave_up = false;
-    for (uint32_t t = t_first; t < tiles && !gave_up; t += t_step) {
-      const Tile ti = tile_at<EPI, CG>(g, t, n_tiles, m_tiles, wn);
+    for (Tiles<EPI, CG> ts(g, wn); ts.more() && !gave_up; ts.next()) {
+      const Tile ti = ts.at();
       const uint32_t k_first = kb_first(ti), k_last = kb_last(ti);
       const bool any_k = k_first < k_last;
       const uint32_t row0 = ti.m0 + rank * BM + quad * 32;  // this warp's rows
-      const float xs = g.x_scale && row0 + lane < g.m ? g.x_scale[row0 + lane] : 1.0f;
       const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-      // asks for the chunk of the residual / upstream gradient at col0; every
-      // lane is done with the one before
-      auto ask = [&](uint32_t col0) {
-        if (lane == 0) {
+      // Asks for 32 columns (f32: 16) of the residual / upstream gradient into
+      // slot 0.  Every lane is done with what was there, every store has read it.
+      auto ask = [&](uint32_t col) {
+        if (g.tma_in && lane == 0 && col < g.n) {
+          stores_read<0>();
           fence_async();
-          mbar_expect_tx(in_bar, in_bytes);
-          tma_load_2d<1>(s_addr(in_slot), &maps.in, (int)col0, (int)row0, in_bar);
+          mbar_expect_tx(in_bar, SLOT_BYTES);
+          tma_load_2d<1>(s_addr(slots), &maps.in, (int)col, (int)row0, in_bar);
         }
       };
-      if (g.tma_in && ti.n0 + half * 32 < g.n && half * 32 < wn) ask(ti.n0 + half * 32);
-      // f(j, value) over this lane's row of the chunk at col0; `next` is the
-      // chunk after it (or >= g.n)
-      auto take = [&](uint32_t col0, uint32_t next, auto f) {
-        if (g.tma_in) {
-          if (!mbar_wait(in_bar, in_ph, abort_flag, g.err, 74)) gave_up = true;
-          in_ph ^= 1u;
-          each_of_row(in_slot, lane, g.other_type, f);
+      auto asked = [&]() {
+        if (!mbar_wait(in_bar, in_ph, abort_flag, g.err, 74)) gave_up = true;
+        in_ph ^= 1u;
+      };
+      // f(first column, 8 values) for this lane's row of the chunk at col0, eight
+      // columns at a time; the first of it was asked for
+      auto take = [&](uint32_t col0, auto f) {
+        if (g.tma_in && g.other_type != BGNN_F32) {
+          asked();
+#pragma unroll
+          for (int u = 0; u < 4; u++) {
+            float o[8];
+            unit16(*slot_unit(slots, lane, u), g.other_type, o);
+            f(8 * u, o);
+          }
           __syncwarp();
-          if (next < g.n) ask(next);
+        } else if (g.tma_in) {
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            if (h == 0 || col0 + 16 < g.n) {
+              if (h == 1) ask(col0 + 16);
+              asked();
+#pragma unroll
+              for (int u = 0; u < 2; u++) {
+                const uint4 a = *slot_unit(slots, lane, 2 * u), b = *slot_unit(slots, lane, 2 * u + 1);
+                const float o[8] = {__uint_as_float(a.x), __uint_as_float(a.y), __uint_as_float(a.z),
+                                    __uint_as_float(a.w), __uint_as_float(b.x), __uint_as_float(b.y),
+                                    __uint_as_float(b.z), __uint_as_float(b.w)};
+                f(16 * h + 8 * u, o);
+              }
+              __syncwarp();
+            }
+          }
         } else {  // rows that TMA cannot take: plain reads along rows, turned round
-          float4 w[8];
+          if (lane == 0) stores_read<0>();
+          __syncwarp();
 #pragma unroll
           for (int i = 0; i < 8; i++) {
             const int r = i * 4 + (lane >> 3), u = lane & 7;
             const uint32_t row = row0 + r, col = col0 + u * 4;
-            w[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float4 w = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (row < g.m && col < g.n)
-              w[i] = load4_row(g.other, g.other_type, (uint64_t)row * g.ld_other + col, g.n - col,
-                               vec_other);
+              w = load4_row(g.other, g.other_type, (uint64_t)row * g.ld_other + col, g.n - col,
+                            vec_other);
+            *turn_unit(slots, r, u) = w;
           }
           __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 8; i++) *turn_unit(in_slot, i * 4 + (lane >> 3), lane & 7) = w[i];
-          __syncwarp();
-          each_of_row(in_slot, lane, BGNN_F32, f);
-        }
-      };
-      // a chunk out, a row a lane
-      auto give = [&](const float (&v)[32], uint32_t col0, int which, int type, uint32_t out_row) {
-        if (g.tma_out) {
-          uint8_t* slot = out_slot;
-          if (type != BGNN_F32) {
-            slot += out_at * 2048;
-            out_at ^= 1u;
-            if (lane == 0) stores_read<1>();
-          } else {
-            if (lane == 0) stores_read<0>();
+          for (int u = 0; u < 4; u++) {
+            const float4 a = *turn_unit(slots, lane, 2 * u), b = *turn_unit(slots, lane, 2 * u + 1);
+            const float o[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            f(8 * u, o);
           }
           __syncwarp();
-          put_row(slot, lane, type, v);
-          fence_async();
-          __syncwarp();
-          if (lane == 0 && row0 < g.m)
-            tma_store_2d(&maps.out[which], (int)col0, (int)out_row, s_addr(slot));
+        }
+      };
+      // a chunk out, a row a lane, through the slots in turn
+      auto give = [&](const float (&v)[32], uint32_t col0, int which, int type, uint32_t out_row) {
+        if (g.tma_out) {
+          auto slot_free = [&]() {
+            if (lane == 0) stores_read<1>();
+            __syncwarp();
+            return slots + out_at * SLOT_BYTES;
+          };
+          auto slot_out = [&](void* slot, uint32_t col) {
+            fence_async();
+            __syncwarp();
+            if (lane == 0 && row0 < g.m && col < g.n)
+              tma_store_2d(&maps.out[which], (int)col, (int)out_row, s_addr(slot));
+            out_at ^= 1u;
+          };
+          if (type == BGNN_F32) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              void* slot = slot_free();
+#pragma unroll
+              for (int u = 0; u < 4; u++)
+                *slot_unit(slot, lane, u) = make_uint4(
+                    __float_as_uint(v[16 * h + 4 * u]), __float_as_uint(v[16 * h + 4 * u + 1]),
+                    __float_as_uint(v[16 * h + 4 * u + 2]), __float_as_uint(v[16 * h + 4 * u + 3]));
+              slot_out(slot, col0 + 16 * h);
+            }
+          } else {
+            void* slot = slot_free();
+            if (type == BGNN_BF16) put_row16<BGNN_BF16>(slot, lane, v);
+            else put_row16<BGNN_F16>(slot, lane, v);
+            slot_out(slot, col0);
+          }
         } else {
           __syncwarp();
-          put_row(out_slot, lane, BGNN_F32, v);
+#pragma unroll
+          for (int u = 0; u < 8; u++)
+            *turn_unit(slots, lane, u) =
+                make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
           __syncwarp();
 #pragma unroll
           for (int i = 0; i < 8; i++) {
@@ -835,14 +881,16 @@ __global__ void __launch_bounds__(THREADS, 1)
             const uint32_t row = row0 + r, col = col0 + u * 4;
             if (row < g.m && col < g.n)
               store4_row(g.out[which], type, (uint64_t)row * g.ld_out + col, g.n - col, vec_out,
-                         *turn_unit(out_slot, r, u));
+                         *turn_unit(slots, r, u));
           }
+          __syncwarp();
         }
       };
       // scales and bias of a chunk: lane j holds column j's
       auto scaled = [&](float (&v)[32], uint32_t col0, int i) {
         const bool in = col0 + lane < g.n;
         if (g.x_scale) {
+          const float xs = row0 + lane < g.m ? g.x_scale[row0 + lane] : 1.0f;
           const float ws = in ? g.w_scale[i][col0 + lane] : 0.0f;
 #pragma unroll
           for (int j = 0; j < 32; j++) v[j] *= xs * __shfl_sync(0xffffffffu, ws, j);
@@ -853,7 +901,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int j = 0; j < 32; j++) v[j] += __shfl_sync(0xffffffffu, bv, j);
         }
       };
-      auto linear_out = [&](float (&v)[32], uint32_t col0, uint32_t next) {
+      auto linear_out = [&](float (&v)[32], uint32_t col0) {
         scaled(v, col0, 0);
         if (g.act != BGNN_ACT_NONE)
           with_act(g.act, [&](auto act) {
@@ -864,16 +912,20 @@ __global__ void __launch_bounds__(THREADS, 1)
               v[j + 1] = f.y;
             }
           });
-        if (g.other) take(col0, next, [&](int j, float o) { v[j] += o; });
+        if (g.other)
+          take(col0, [&](int j0, const float (&o)[8]) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j0 + j] += o[j];
+          });
         give(v, col0, 0, g.out_type, row0);
       };
-      auto after = [&](uint32_t c) { return c + 64 < wn ? ti.n0 + c + 64 : g.n; };
 
+      if (group * 32 < wn) ask(ti.n0 + group * 32);
       if constexpr (EPI == EPI_LINEAR_F32) {
         // pieces of the contraction added in f32 registers, rounded to nearest
-        float sum[4][32];
+        float sum[2][32];
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < 2; i++)
 #pragma unroll
           for (int j = 0; j < 32; j++) sum[i][j] = 0.0f;
         uint32_t kb = k_first;
@@ -885,8 +937,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           tc_fence_after();
           const uint32_t acc = tmem + lanes + buf * g.bn;
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const uint32_t c = half * 32 + i * 64;
+          for (int i = 0; i < 2; i++) {
+            const uint32_t c = group * 32 + i * 128;
             if (c < wn && any_k) {
               float v[32];
               tmem_ld32(acc + c, v);
@@ -900,17 +952,21 @@ __global__ void __launch_bounds__(THREADS, 1)
         } while (kb < k_last);
         if (gave_up) break;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const uint32_t c = half * 32 + i * 64;
-          if (c < wn && ti.n0 + c < g.n) linear_out(sum[i], ti.n0 + c, after(c));
+        for (int i = 0; i < 2; i++) {
+          const uint32_t c = group * 32 + i * 128;
+          if (c < wn && ti.n0 + c < g.n) {
+            if (i) ask(ti.n0 + c);
+            linear_out(sum[i], ti.n0 + c);
+          }
         }
       } else {
         if (!mbar_wait(b_accf + 8 * buf, aph, abort_flag, g.err, 73)) break;
         tc_fence_after();
         const uint32_t acc = tmem + lanes + buf * g.bn;
-        for (uint32_t c = half * 32; c < wn; c += 64) {
+        for (uint32_t c = group * 32; c < wn; c += 128) {
           const uint32_t col0 = ti.n0 + c;
           if (col0 >= g.n) break;  // uniform: the chunk is past the last column
+          if (c >= 128) ask(col0);
           float v[32], u[32];      // u: the second product's
           tmem_ld32(acc + c, v);
           if constexpr (TWO) tmem_ld32(acc + wn + c, u);
@@ -924,7 +980,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
           }
           if constexpr (EPI == EPI_LINEAR) {
-            linear_out(v, col0, after(c));
+            linear_out(v, col0);
           } else if constexpr (EPI == EPI_PARTIAL) {
             if (parts)
               give(v, col0, 0, BGNN_F32,
@@ -933,16 +989,19 @@ __global__ void __launch_bounds__(THREADS, 1)
               give(v, col0, (int)ti.batch, g.out_type, row0);
           } else if constexpr (EPI == EPI_LINEAR_BWD) {
             scaled(v, col0, 0);
-            float o[32];
-            take(col0, after(c), [&](int j, float w) { o[j] = w; });
+            // act' first, the gradient on top
             with_act(g.act, [&](auto act) {
 #pragma unroll
               for (int j = 0; j < 32; j += 2) {
                 float2 f0, f1;
                 act_grad_two<decltype(act)::value>(make_float2(v[j], v[j + 1]), g.act_p, f0, f1);
-                v[j] = o[j] * f0.y;
-                v[j + 1] = o[j + 1] * f1.y;
+                v[j] = f0.y;
+                v[j + 1] = f1.y;
               }
+            });
+            take(col0, [&](int j0, const float (&o)[8]) {
+#pragma unroll
+              for (int j = 0; j < 8; j++) v[j0 + j] *= o[j];
             });
             give(v, col0, 0, g.out_type, row0);
           } else if constexpr (EPI == EPI_GATED) {
@@ -962,17 +1021,22 @@ __global__ void __launch_bounds__(THREADS, 1)
           } else {
             scaled(v, col0, 0);
             scaled(u, col0, 1);
-            float o[32];
-            take(col0, after(c), [&](int j, float w) { o[j] = w; });
             with_act(g.act, [&](auto act) {
 #pragma unroll
               for (int j = 0; j < 32; j += 2) {
                 float2 f0, f1;
                 act_grad_two<decltype(act)::value>(make_float2(v[j], v[j + 1]), g.act_p, f0, f1);
-                v[j] = o[j] * u[j] * f0.y;  // dg
-                v[j + 1] = o[j + 1] * u[j + 1] * f1.y;
-                u[j] = o[j] * f0.x;  // du
-                u[j + 1] = o[j + 1] * f1.x;
+                v[j] = u[j] * f0.y;  // dg / grad
+                v[j + 1] = u[j + 1] * f1.y;
+                u[j] = f0.x;  // du / grad
+                u[j + 1] = f1.x;
+              }
+            });
+            take(col0, [&](int j0, const float (&o)[8]) {
+#pragma unroll
+              for (int j = 0; j < 8; j++) {
+                v[j0 + j] *= o[j];
+                u[j0 + j] *= o[j];
               }
             });
             give(v, col0, 0, g.out_type, row0);
@@ -1093,23 +1157,20 @@ bool tma_takes(int type, const Mat& x) {
          x.rows < (1ull << 31);
 }
 
-// 32 x 32 boxes of f32 (128-byte swizzle) or 16-bit (64-byte) elements: the
-// epilogue's chunks
+// boxes of 64 bytes x 32 rows, 64-byte swizzle: the epilogue's slots
 int make_chunk_map(bgnn_ctx* ctx, CUtensorMap* map, int type, const Mat& x) {
   auto enc = encode_fn();
   if (!enc) return bgnn_set_error(ctx, BGNN_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled unavailable");
   cuuint64_t dims[2] = {x.cols, x.rows};
   cuuint64_t strides[1] = {x.ld * dtype_size(type)};
-  cuuint32_t box[2] = {32, 32};
+  cuuint32_t box[2] = {type == BGNN_F32 ? 16u : 32u, 32};
   cuuint32_t el[2] = {1, 1};
   const CUtensorMapDataType dt = type == BGNN_BF16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                  : type == BGNN_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   const CUresult r =
       enc(map, dt, 2, const_cast<void*>(x.p), dims, strides, box, el,
-          CU_TENSOR_MAP_INTERLEAVE_NONE,
-          type == BGNN_F32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-          CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return bgnn_set_error(ctx, BGNN_ERR_UNSUPPORTED, "tensor map encode failed (%d)", (int)r);
   return BGNN_OK;
