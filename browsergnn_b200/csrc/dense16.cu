@@ -21,10 +21,9 @@
 //   warp 17   MMA issuer (one thread): tcgen05.mma, M = 128, N = BN, into one
 //             of two tensor-memory accumulators;
 //   warps 0-15 epilogue: warp w takes the accumulator lanes (rows) of its
-//             quadrant w % 4 and every fourth 32-column chunk; chunks come in
-//             and go out by TMA through two shared-memory slots a warp, or,
-//             where TMA cannot take the rows, turned round there and read and
-//             written along rows.  Sixteen warps, four a scheduler: with eight
+//             quadrant w % 4 and every fourth 32-column chunk; a chunk of the
+//             residual comes by TMA into one shared-memory slot, the result
+//             goes out through the other, turned round to run along rows.  Sixteen warps, four a scheduler: with eight
 //             the activations of a short contraction ran at a third of the
 //             issue rate and bound the kernel.
 // An operand whose contraction runs down its rows (w in dx, both in dw) is
@@ -73,10 +72,10 @@ constexpr uint32_t MAX_PER = 512;  // k blocks of a dw range
 
 // One contraction segment: A [m, k] and B [n, k] tiles of one or two tensors.
 // Where `b1` is used (gated), B's tile is rows of b0 above rows of b1.
-// in / out: the residual or upstream gradient and the outputs in boxes of a slot,
-// where TMA can take them.
+// in: the residual or upstream gradient in boxes of a slot, where TMA can take
+// it.
 struct Maps {
-  CUtensorMap a[2], b[2], in, out[2];
+  CUtensorMap a[2], b[2], in;
 };
 
 struct GemmArgs {
@@ -103,8 +102,8 @@ struct GemmArgs {
   int out_type;
   void* out[2];           // gated backward: dg and du; dw: one a batch
   uint64_t ld_out;
-  int tma_in, tma_out;    // maps.in, maps.out are set
-  uint32_t part_rows;     // EPI_PARTIAL: rows of a partial matrix (0: dw whole, no parts)
+  int tma_in;             // maps.in is set
+  float* part;            // EPI_PARTIAL: [splits, batches, m, ld_out]; NULL: dw whole, no parts
   int* err;
 };
 
@@ -483,23 +482,6 @@ __device__ __forceinline__ float4* turn_unit(void* slots, int row, int unit) {
   return reinterpret_cast<float4*>(static_cast<char*>(slots) + row * 128 +
                                    ((unit ^ (row & 7)) << 4));
 }
-__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, uint32_t src) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
-          reinterpret_cast<uint64_t>(map)),
-      "r"(x), "r"(y), "r"(src)
-      : "memory");
-  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-}
-// all but N of this thread's stores have read their shared memory
-template <int N>
-__device__ __forceinline__ void stores_read() {
-  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
-}
-// this thread's stores are done
-__device__ __forceinline__ void stores_done() {
-  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-}
 __device__ __forceinline__ void fence_async() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
@@ -524,28 +506,15 @@ __device__ __forceinline__ float4 load4_row(const void* p, int dt, uint64_t i, u
   if (left > 3) v.w = load_any(p, dt, i + 3);
   return v;
 }
-__device__ __forceinline__ void store4_row(void* p, int dt, uint64_t i, uint32_t left, bool vec,
-                                           float4 v) {
-  if (vec && left >= 4) {
-    if (dt == BGNN_F32) {
-      *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = v;
-    } else {
-      const uint2 w = dt == BGNN_BF16
-                          ? make_uint2(pack2<BGNN_BF16>(v.x, v.y), pack2<BGNN_BF16>(v.z, v.w))
-                          : make_uint2(pack2<BGNN_F16>(v.x, v.y), pack2<BGNN_F16>(v.z, v.w));
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = w;
-    }
-    return;
-  }
-  if (left > 0) store_any(p, dt, i, v.x);
-  if (left > 1) store_any(p, dt, i + 1, v.y);
-  if (left > 2) store_any(p, dt, i + 2, v.z);
-  if (left > 3) store_any(p, dt, i + 3, v.w);
-}
 // whether four elements at (row stride ld, column a multiple of 4) are one access
 __device__ __forceinline__ bool vec4_ok(const void* p, int dt, uint64_t ld) {
   const uint32_t b = dt == BGNN_F32 ? 16u : 8u;
   return ((uintptr_t)p & (b - 1)) == 0 && ld % 4 == 0;
+}
+
+// whether 16 bytes of a row, from a multiple of as many, are one access
+__device__ __forceinline__ bool vec16_ok(const void* p, int dt, uint64_t ld) {
+  return ((uintptr_t)p & 15u) == 0 && ld % (dt == BGNN_F32 ? 4 : 8) == 0;
 }
 
 // the tiles of a CTA (pair), columns fastest
@@ -751,10 +720,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int quad = warp & 3, group = warp >> 2;  // rows; every fourth 32-column chunk
     uint8_t* slots = gbase + RING_BYTES + warp * WARP_BYTES;
     const uint32_t in_bar = b_in + 8 * warp;
-    uint32_t buf = 0, aph = 0, in_ph = 0, out_at = 1;
-    const bool parts = EPI == EPI_PARTIAL && g.part_rows;
-    const bool vec_out = vec4_ok(g.out[0], g.out_type, g.ld_out) &&
-                         (!g.out[1] || vec4_ok(g.out[1], g.out_type, g.ld_out));
+    uint32_t buf = 0, aph = 0, in_ph = 0;
+    const bool vec_out = EPI == EPI_PARTIAL && g.part
+                             ? g.ld_out % 4 == 0
+                             : vec16_ok(g.out[0], g.out_type, g.ld_out) &&
+                                   (!g.out[1] || vec16_ok(g.out[1], g.out_type, g.ld_out));
     const bool vec_other = g.other && vec4_ok(g.other, g.other_type, g.ld_other);
     // hands the accumulator back once every lane has read it
     auto release = [&]() {
@@ -771,10 +741,9 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint32_t row0 = ti.m0 + rank * BM + quad * 32;  // this warp's rows
       const uint32_t lanes = (uint32_t)(quad * 32) << 16;
       // Asks for 32 columns (f32: 16) of the residual / upstream gradient into
-      // slot 0.  Every lane is done with what was there, every store has read it.
+      // slot 0, with which every lane is done.
       auto ask = [&](uint32_t col) {
         if (g.tma_in && lane == 0 && col < g.n) {
-          stores_read<0>();
           fence_async();
           mbar_expect_tx(in_bar, SLOT_BYTES);
           tma_load_2d<1>(s_addr(slots), &maps.in, (int)col, (int)row0, in_bar);
@@ -814,8 +783,6 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
           }
         } else {  // rows that TMA cannot take: plain reads along rows, turned round
-          if (lane == 0) stores_read<0>();
-          __syncwarp();
 #pragma unroll
           for (int i = 0; i < 8; i++) {
             const int r = i * 4 + (lane >> 3), u = lane & 7;
@@ -836,54 +803,53 @@ __global__ void __launch_bounds__(THREADS, 1)
           __syncwarp();
         }
       };
-      // a chunk out, a row a lane, through the slots in turn
-      auto give = [&](const float (&v)[32], uint32_t col0, int which, int type, uint32_t out_row) {
-        if (g.tma_out) {
-          auto slot_free = [&]() {
-            if (lane == 0) stores_read<1>();
-            __syncwarp();
-            return slots + out_at * SLOT_BYTES;
-          };
-          auto slot_out = [&](void* slot, uint32_t col) {
-            fence_async();
-            __syncwarp();
-            if (lane == 0 && row0 < g.m && col < g.n)
-              tma_store_2d(&maps.out[which], (int)col, (int)out_row, s_addr(slot));
-            out_at ^= 1u;
-          };
-          if (type == BGNN_F32) {
+      // Out, a row a lane: through slot 1, turned round, so that four lanes
+      // write the 64 bytes of a row.  (TMA stores of a slot took turns with the
+      // ring's loads: one engine, about 2.6 clocks a row of either.)
+      auto give_slot = [&](void* out, uint64_t ld, int type, uint32_t col) {
+        void* slot = slots + SLOT_BYTES;
+        __syncwarp();
+        const uint32_t per = type == BGNN_F32 ? 4u : 8u;  // elements of a unit
+        const uint32_t c = col + (lane & 3) * per;
+        const uint32_t n = c < g.n ? g.n - c : 0u;
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-              void* slot = slot_free();
-#pragma unroll
-              for (int u = 0; u < 4; u++)
-                *slot_unit(slot, lane, u) = make_uint4(
-                    __float_as_uint(v[16 * h + 4 * u]), __float_as_uint(v[16 * h + 4 * u + 1]),
-                    __float_as_uint(v[16 * h + 4 * u + 2]), __float_as_uint(v[16 * h + 4 * u + 3]));
-              slot_out(slot, col0 + 16 * h);
-            }
+        for (int i = 0; i < 4; i++) {
+          const int r = i * 8 + (lane >> 2);
+          const uint4 q = *slot_unit(slot, r, lane & 3);
+          if (row0 + r >= g.m || n == 0) continue;
+          const uint64_t at = (uint64_t)(row0 + r) * ld + c;
+          if (vec_out && n >= per) {
+            *reinterpret_cast<uint4*>(static_cast<char*>(out) + at * (16u / per)) = q;
           } else {
-            void* slot = slot_free();
-            if (type == BGNN_BF16) put_row16<BGNN_BF16>(slot, lane, v);
-            else put_row16<BGNN_F16>(slot, lane, v);
-            slot_out(slot, col0);
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++)
+              if (j < per && j < n) {
+                if (type == BGNN_F32) {
+                  if (j < 4) static_cast<uint32_t*>(out)[at + j] = w[j & 3];
+                } else {
+                  static_cast<uint16_t*>(out)[at + j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+                }
+              }
+          }
+        }
+        __syncwarp();
+      };
+      auto give = [&](const float (&v)[32], uint32_t col0, void* out, uint64_t ld, int type) {
+        if (type == BGNN_F32) {
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+              *slot_unit(slots + SLOT_BYTES, lane, u) = make_uint4(
+                  __float_as_uint(v[16 * h + 4 * u]), __float_as_uint(v[16 * h + 4 * u + 1]),
+                  __float_as_uint(v[16 * h + 4 * u + 2]), __float_as_uint(v[16 * h + 4 * u + 3]));
+            give_slot(out, ld, type, col0 + 16 * h);
           }
         } else {
-          __syncwarp();
-#pragma unroll
-          for (int u = 0; u < 8; u++)
-            *turn_unit(slots, lane, u) =
-                make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const int r = i * 4 + (lane >> 3), u = lane & 7;
-            const uint32_t row = row0 + r, col = col0 + u * 4;
-            if (row < g.m && col < g.n)
-              store4_row(g.out[which], type, (uint64_t)row * g.ld_out + col, g.n - col, vec_out,
-                         *turn_unit(slots, r, u));
-          }
-          __syncwarp();
+          if (type == BGNN_BF16) put_row16<BGNN_BF16>(slots + SLOT_BYTES, lane, v);
+          else put_row16<BGNN_F16>(slots + SLOT_BYTES, lane, v);
+          give_slot(out, ld, type, col0);
         }
       };
       // scales and bias of a chunk: lane j holds column j's
@@ -917,7 +883,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int j = 0; j < 8; j++) v[j0 + j] += o[j];
           });
-        give(v, col0, 0, g.out_type, row0);
+        give(v, col0, g.out[0], g.ld_out, g.out_type);
       };
 
       if (group * 32 < wn) ask(ti.n0 + group * 32);
@@ -982,11 +948,12 @@ __global__ void __launch_bounds__(THREADS, 1)
           if constexpr (EPI == EPI_LINEAR) {
             linear_out(v, col0);
           } else if constexpr (EPI == EPI_PARTIAL) {
-            if (parts)
-              give(v, col0, 0, BGNN_F32,
-                   row0 + (ti.split * g.batches + ti.batch) * g.part_rows);
+            if (g.part)
+              give(v, col0,
+                   g.part + ((uint64_t)ti.split * g.batches + ti.batch) * g.m * g.ld_out, g.ld_out,
+                   BGNN_F32);
             else
-              give(v, col0, (int)ti.batch, g.out_type, row0);
+              give(v, col0, ti.batch ? g.out[1] : g.out[0], g.ld_out, g.out_type);
           } else if constexpr (EPI == EPI_LINEAR_BWD) {
             scaled(v, col0, 0);
             // act' first, the gradient on top
@@ -1003,7 +970,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
               for (int j = 0; j < 8; j++) v[j0 + j] *= o[j];
             });
-            give(v, col0, 0, g.out_type, row0);
+            give(v, col0, g.out[0], g.ld_out, g.out_type);
           } else if constexpr (EPI == EPI_GATED) {
             scaled(v, col0, 0);
             scaled(u, col0, 1);
@@ -1017,7 +984,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 v[j + 1] = f.y;
               }
             });
-            give(v, col0, 0, g.out_type, row0);
+            give(v, col0, g.out[0], g.ld_out, g.out_type);
           } else {
             scaled(v, col0, 0);
             scaled(u, col0, 1);
@@ -1039,14 +1006,13 @@ __global__ void __launch_bounds__(THREADS, 1)
                 u[j0 + j] *= o[j];
               }
             });
-            give(v, col0, 0, g.out_type, row0);
-            give(u, col0, 1, g.out_type, row0);
+            give(v, col0, g.out[0], g.ld_out, g.out_type);
+            give(u, col0, g.out[1], g.ld_out, g.out_type);
           }
         }
         release();
       }
     }
-    if (lane == 0) stores_done();
   }
   pair_sync<CG>();
   if (warp == EPI_WARPS) {
@@ -1055,19 +1021,19 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
-// dw: the splits' partial matrices (prows rows of ld f32 each) added in order
+// dw: the splits' partial matrices (rows ld f32 apart) added in order
 __global__ void __launch_bounds__(256) k_add_splits(const float* __restrict__ part, uint32_t splits,
-                                                    uint32_t batches, uint32_t prows, uint32_t ld,
+                                                    uint32_t batches, uint32_t ld,
                                                     uint32_t rows, uint32_t cols, void* out0,
                                                     void* out1, int out_type) {
   const uint64_t mn = (uint64_t)rows * cols, total = mn * batches;
-  const uint64_t step = (uint64_t)prows * ld * batches;
+  const uint64_t step = (uint64_t)rows * ld * batches;
   for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
        i += (uint64_t)gridDim.x * blockDim.x) {
     const uint32_t b = i >= mn;
     const uint64_t e = b ? i - mn : i;
     const uint32_t r = (uint32_t)(e / cols), c = (uint32_t)(e - (uint64_t)r * cols);
-    const float* p = part + ((uint64_t)b * prows + r) * ld + c;
+    const float* p = part + ((uint64_t)b * rows + r) * ld + c;
     float v = *p;
     for (uint32_t s = 1; s < splits; s++) v += p[s * step];
     store_any(b ? out1 : out0, out_type, e, v);
@@ -1175,8 +1141,8 @@ int make_chunk_map(bgnn_ctx* ctx, CUtensorMap* map, int type, const Mat& x) {
     return bgnn_set_error(ctx, BGNN_ERR_UNSUPPORTED, "tensor map encode failed (%d)", (int)r);
   return BGNN_OK;
 }
-// maps.in and maps.out of a product [m, n] where TMA can take them
-int make_chunk_maps(bgnn_ctx* ctx, Maps* maps, GemmArgs* g) {
+// maps.in of a product [m, n] where TMA can take it
+int make_in_map(bgnn_ctx* ctx, Maps* maps, GemmArgs* g) {
   g->tma_in = 0;
   if (g->other) {
     const Mat in = {g->other, g->m, g->n, g->ld_other};
@@ -1185,16 +1151,6 @@ int make_chunk_maps(bgnn_ctx* ctx, Maps* maps, GemmArgs* g) {
       g->tma_in = 1;
     }
   }
-  g->tma_out = 1;
-  // a TMA store writes whole 16-byte units: the columns behind a row that ends
-  // inside one would be lost
-  if (g->n * dtype_size(g->out_type) % 16) g->tma_out = 0;
-  for (int i = 0; i < 2; i++)
-    if (g->out[i] && !tma_takes(g->out_type, {g->out[i], g->m, g->n, g->ld_out})) g->tma_out = 0;
-  for (int i = 0; i < 2 && g->tma_out; i++)
-    if (g->out[i])
-      BGNN_TRY(make_chunk_map(ctx, &maps->out[i], g->out_type,
-                              {g->out[i], g->m, g->n, g->ld_out}));
   return BGNN_OK;
 }
 
@@ -1316,7 +1272,7 @@ int run_nt(bgnn_ctx* ctx, GemmArgs& g, Mat x, const Mat (&w)[2], uint32_t k) {
       BGNN_TRY(make_map(ctx, &maps.b[i], g.in_type, wi, TWO ? g.bn / 2 : g.bn / sh.cg));
     }
   }
-  BGNN_TRY(make_chunk_maps(ctx, &maps, &g));
+  BGNN_TRY(make_in_map(ctx, &maps, &g));
   if constexpr (EPI == EPI_LINEAR)
     if (g.out_type == BGNN_F32) return launch<EPI_LINEAR_F32>(ctx, maps, g, sh);
   return launch<EPI>(ctx, maps, g, sh);
@@ -1347,7 +1303,6 @@ int run_dx(bgnn_ctx* ctx, int type, uint32_t m, uint32_t n, uint32_t k, const Ma
   g.out_type = type;
   g.out[0] = dx;
   g.ld_out = k;
-  BGNN_TRY(make_chunk_maps(ctx, &maps, &g));
   return launch<EPI_LINEAR>(ctx, maps, g, sh);
 }
 
@@ -1390,22 +1345,14 @@ int run_dw(bgnn_ctx* ctx, int type, uint32_t m, uint32_t n, uint32_t k, const Ma
   g.out[0] = dw[0];
   g.out[1] = dw[1];
   g.ld_out = k;
-  if (g.splits == 1) {
-    BGNN_TRY(make_chunk_maps(ctx, &maps, &g));
-    return launch<EPI_PARTIAL>(ctx, maps, g, sh);
-  }
-  // whole tiles of rows, so that a tile's last rows stay in its own part
-  g.part_rows = blocks_of(n, BM * sh.cg) * BM * sh.cg;
-  const uint32_t ldp = (k + 3) / 4 * 4;
-  const uint64_t prows = (uint64_t)g.part_rows * terms * g.splits;
-  BGNN_REQUIRE(ctx, prows < (1ull << 31), "weight gradient of %u x %u: too many parts", n, k);
-  BGNN_TRY(bgnn_tmp_alloc(ctx, part, prows * ldp * sizeof(float)));
-  g.tma_out = 1;
-  BGNN_TRY(make_chunk_map(ctx, &maps.out[0], BGNN_F32, {part.p, prows, k, ldp}));
+  if (g.splits == 1) return launch<EPI_PARTIAL>(ctx, maps, g, sh);
+  g.ld_out = (k + 3) / 4 * 4;
+  BGNN_TRY(bgnn_tmp_alloc(ctx, part, (uint64_t)n * g.ld_out * terms * g.splits * sizeof(float)));
+  g.part = part.as<float>();
   BGNN_TRY(launch<EPI_PARTIAL>(ctx, maps, g, sh));
   const uint64_t want = ((uint64_t)n * k * terms + 255) / 256, cap = (uint64_t)ctx->num_sms * 16;
   k_add_splits<<<(unsigned)(want < cap ? want : cap), 256, 0, ctx->stream>>>(
-      part.as<float>(), g.splits, (uint32_t)terms, g.part_rows, ldp, n, k, dw[0], dw[1], type);
+      g.part, g.splits, (uint32_t)terms, (uint32_t)g.ld_out, n, k, dw[0], dw[1], type);
   BGNN_LAUNCHED(ctx);
   return BGNN_OK;
 }
