@@ -8,13 +8,17 @@
 // and, for the gradients g_l of logp_t and g_h of H,
 //   dx_j = p_j (-g_l - g_h (log p_j + H)) + g_l [j = t],   p_j = exp(x_j - lse).
 //
-// One pass: every thread keeps a running (m, S, W = sum (x - m) exp(x - m))
-// in f32 and rescales it when its maximum moves (W' = e^(m-m') (W + (m-m') S));
-// pairs merge the same way.  The top list lives sorted in a warp's lanes
-// (lane i: the i-th best); an element enters when it beats the last of the
-// list, so after the first few hundred elements the test is one comparison a
-// vector.  A long row is split over blocks and joined by k_logp_join; short
-// rows take a warp each.  Memory bound: the logits (and masks) are read once.
+// One pass: every thread keeps a running (m, S, W = sum a 2^a), a = (x - m)
+// log2(e), in f32 and rescales it when its maximum moves (W' = 2^d (W + d S));
+// pairs merge the same way.  The k-th largest of a block's 256 thread maxima is
+// at most the row's k-th largest logit, so the top list is among the elements
+// that reach it: about k of them, in the vectors of the threads whose maximum
+// does, which are read once more (from L2) and ranked by counting.  (Keeping
+// the list sorted in a warp's lanes while reading took 565 us instead of 177
+// without a list, 8,192 x 32,000 bf16, k = 20; it is what a row with hundreds
+// of equal logits at the border falls back to.)  A long row is split over blocks
+// and joined by k_logp_join; short rows take a warp each.  Memory bound: the
+// logits (and masks) are read once.
 #include "lowp.cuh"
 
 namespace {
@@ -43,6 +47,21 @@ struct LogpArgs {
   int* err;
 };
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+// An exponent on its way into 2^a and a 2^a: not below -150, where 2^a is 0, so
+// that a 2^a is never -inf * 0 (x - m may be -inf beside a mask of the type's
+// lowest value).  NaN stays NaN.
+__device__ __forceinline__ float exponent(float d) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(d * LOG2E), "f"(-150.0f));
+  return r;
+}
+
 struct Stat {
   float m, s, w;
 };
@@ -51,15 +70,13 @@ __device__ __forceinline__ Stat stat_merge(Stat a, Stat b) {
   const float m = fmaxf(a.m, b.m);
   const float ms = m == -INFINITY ? 0.0f : m;
   // the side with nothing in it contributes S = W = 0 whatever its m
-  const float da = a.m == -INFINITY ? 0.0f : a.m - ms, db = b.m == -INFINITY ? 0.0f : b.m - ms;
-  const float ea = __expf(da), eb = __expf(db);
-  const float sa = a.s * ea, sb = b.s * eb;
+  const float da = a.m == -INFINITY ? 0.0f : exponent(a.m - ms);
+  const float db = b.m == -INFINITY ? 0.0f : exponent(b.m - ms);
+  const float ea = ex2(da), eb = ex2(db);
   Stat r;
   r.m = m;
-  r.s = sa + sb;
-  // da * sa only while sa is not 0: da may be as low as -inf (a row of the
-  // type's lowest value beside an ordinary one)
-  r.w = a.w * ea + b.w * eb + (sa != 0.0f ? da * sa : 0.0f) + (sb != 0.0f ? db * sb : 0.0f);
+  r.s = a.s * ea + b.s * eb;
+  r.w = (a.w + da * a.s) * ea + (b.w + db * b.s) * eb;
   return r;
 }
 
@@ -146,62 +163,136 @@ __device__ __forceinline__ void stat_add(Stat& t, const float (&v)[8]) {
 #pragma unroll
   for (int j = 1; j < 8; j++) cm = fmaxf(cm, v[j]);
   if (cm > t.m) {
-    const float d = t.m == -INFINITY ? 0.0f : t.m - cm;
-    const float e = __expf(d);
+    const float d = t.m == -INFINITY ? 0.0f : exponent(t.m - cm);
+    const float e = ex2(d);
+    t.w = (t.w + d * t.s) * e;
     t.s *= e;
-    t.w = t.w * e + (t.s != 0.0f ? d * t.s : 0.0f);
     t.m = cm;
   }
   const float m = t.m == -INFINITY ? 0.0f : t.m;
+  float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
-  for (int j = 0; j < 8; j++) {
-    const float d = v[j] - m;
-    const float e = __expf(d);
-    t.s += e;
-    t.w += d == -INFINITY ? 0.0f : d * e;
+  for (int j = 0; j < 8; j += 2) {
+    const float a0 = exponent(v[j] - m), a1 = exponent(v[j + 1] - m);
+    const float e0 = ex2(a0), e1 = ex2(a1);
+    s0 += e0;
+    s1 += e1;
+    t.w = fmaf(a0, e0, fmaf(a1, e1, t.w));
   }
+  t.s += s0 + s1;
 }
 
-// one row's figures from its statistics and list; one warp
+// a row's log-sum-exp, entropy and log probability from its statistics
 template <int DT>
-__device__ __forceinline__ void finish_row(const LogpArgs& a, uint64_t row, Stat t,
-                                           const TopList& best, int lane) {
+__device__ __forceinline__ void finish_row(const LogpArgs& a, uint64_t row, Stat t) {
   const bool empty = t.m == -INFINITY && t.s == 0.0f;
   // a +inf logit leaves no finite difference: all figures NaN, as for a NaN
   // logit.  x - m first: m + log S alone drops log S beside a large m.
   const float ls = logf(t.s);
-  if (lane == 0) {
-    if (a.lse) a.lse[row] = empty ? -INFINITY : t.m + ls;
-    if (a.entropy) a.entropy[row] = empty ? 0.0f : fmaf(-t.w, __fdiv_rn(1.0f, t.s), ls);
-    if (a.logp) {
-      const uint32_t c = a.targets[row];
-      float lp = 0.0f;  // no choice given
-      if (c != NO_CHOICE) {
-        if (c >= a.cols) {
-          dev_raise(a.err, DEVERR_INDEX, c, 60);
-          lp = __int_as_float(0x7fc00000);
-        } else {
-          const bool out = a.mask && a.mask[row * a.ld_mask + c];
-          const float x = Elt<DT>::get(static_cast<const elt_t<DT>*>(a.x)[row * a.ld + c]);
-          lp = (empty || out) ? -INFINITY : (x - t.m) - ls;
-        }
+  if (a.lse) a.lse[row] = empty ? -INFINITY : t.m + ls;
+  if (a.entropy) a.entropy[row] = empty ? 0.0f : fmaf(-t.w * LN2, __fdiv_rn(1.0f, t.s), ls);
+  if (a.logp) {
+    const uint32_t c = a.targets[row];
+    float lp = 0.0f;  // no choice given
+    if (c != NO_CHOICE) {
+      if (c >= a.cols) {
+        dev_raise(a.err, DEVERR_INDEX, c, 60);
+        lp = __int_as_float(0x7fc00000);
+      } else {
+        const bool out = a.mask && a.mask[row * a.ld_mask + c];
+        const float x = Elt<DT>::get(static_cast<const elt_t<DT>*>(a.x)[row * a.ld + c]);
+        lp = (empty || out) ? -INFINITY : (x - t.m) - ls;
       }
-      a.logp[row] = lp;
+    }
+    a.logp[row] = lp;
+  }
+}
+// entry i of a row's list
+__device__ __forceinline__ void put_top(const LogpArgs& a, uint64_t row, Stat t, int i, float v,
+                                        uint32_t id) {
+  const bool some = v > -INFINITY;
+  a.top_ids[row * a.top + i] = some ? id : NO_CHOICE;
+  a.top_logp[row * a.top + i] = some ? (v - t.m) - logf(t.s) : -INFINITY;
+}
+
+// ---- the top list of a block ---------------------------------------------------
+constexpr int CANDS = 256;  // candidates that are ranked by counting
+struct TopShared {
+  float m[LP_WARPS], s[LP_WARPS], w[LP_WARPS];
+  float v[CANDS];
+  uint32_t id[CANDS];
+  int n;
+};
+// a whole number that orders as the float does; 0: nothing
+__device__ __forceinline__ uint32_t order_key(float v) {
+  if (!(v > -INFINITY)) return 0u;
+  const uint32_t b = __float_as_uint(v + 0.0f);  // -0 as +0
+  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+// A border that at least k of the block's keys reach, and not many more: the
+// k-th largest, or its leading bits.  0 when fewer than k keys are not 0.
+__device__ __forceinline__ uint32_t border(uint32_t key, int k) {
+  uint32_t p = 0;
+  for (int bit = 31; bit >= 0; bit--) {
+    const uint32_t q = p | (1u << bit);
+    const int c = __syncthreads_count(key >= q);
+    if (c >= k) {
+      p = q;
+      if (c <= k + 8) break;
     }
   }
-  if (lane < a.top) {
-    const bool some = best.v > -INFINITY;
-    a.top_ids[row * a.top + lane] = some ? best.id : NO_CHOICE;
-    a.top_logp[row * a.top + lane] = some ? (best.v - t.m) - ls : -INFINITY;
+  return p;
+}
+// appends a candidate a lane; all lanes of the warp call
+__device__ __forceinline__ void add_cands(TopShared& sm, bool in, float v, uint32_t id, int lane) {
+  const uint32_t b = __ballot_sync(0xffffffffu, in);
+  if (b == 0) return;
+  int at = 0;
+  if (lane == 0) at = atomicAdd(&sm.n, __popc(b));  // their order is not kept: they are ranked
+  at = __shfl_sync(0xffffffffu, at, 0) + __popc(b & ((1u << lane) - 1));
+  if (in && at < CANDS) sm.v[at] = v, sm.id[at] = id;
+}
+// the block's statistics, in every thread
+__device__ __forceinline__ Stat block_stat(TopShared& sm, Stat t, int warp, int lane) {
+  t = warp_stat(t);
+  if (lane == 0) sm.m[warp] = t.m, sm.s[warp] = t.s, sm.w[warp] = t.w;
+  __syncthreads();
+  t = {sm.m[0], sm.s[0], sm.w[0]};
+#pragma unroll
+  for (int i = 1; i < LP_WARPS; i++) t = stat_merge(t, {sm.m[i], sm.s[i], sm.w[i]});
+  return t;
+}
+// put(i, v, id) for the list's entries, i ascending over the block's threads
+template <class F>
+__device__ __forceinline__ void rank_cands(const TopShared& sm, int top, F put) {
+  const int n = sm.n;
+  for (int i = threadIdx.x; i < n; i += LP_WARPS * 32) {
+    const float v = sm.v[i];
+    const uint32_t id = sm.id[i];
+    int r = 0;
+    for (int j = 0; j < n; j++) r += before(sm.v[j], sm.id[j], v, id);
+    if (r < top) put(r, v, id);
   }
+  for (int i = n + threadIdx.x; i < top; i += LP_WARPS * 32) put(i, -INFINITY, NO_CHOICE);
+}
+// the warps' sorted lists as one; warp 0 gets it.  Uses sm.v and sm.id.
+__device__ __forceinline__ void join_lists(TopShared& sm, TopList& best, int top, int warp,
+                                           int lane) {
+  static_assert(CANDS == LP_WARPS * TOP_MAX, "a list a warp");
+  __syncthreads();
+  sm.v[warp * TOP_MAX + lane] = best.v;
+  sm.id[warp * TOP_MAX + lane] = best.id;
+  __syncthreads();
+  if (warp == 0)
+    for (int w = 1; w < LP_WARPS; w++)
+      best.offer(lane < top ? sm.v[w * TOP_MAX + lane] : -INFINITY,
+                 lane < top ? sm.id[w * TOP_MAX + lane] : NO_CHOICE, top, lane);
 }
 
 // rows of one segment: block = (row, segment); its warps interleave vectors
 template <int DT>
 __global__ void __launch_bounds__(LP_WARPS * 32) k_logp(const LogpArgs a) {
-  __shared__ float sm_m[LP_WARPS], sm_s[LP_WARPS], sm_w[LP_WARPS];
-  __shared__ float sm_v[LP_WARPS][TOP_MAX];
-  __shared__ uint32_t sm_id[LP_WARPS][TOP_MAX];
+  __shared__ TopShared sm;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint64_t row = blockIdx.x / a.splits;
   const uint32_t split = blockIdx.x % a.splits;
@@ -214,87 +305,123 @@ __global__ void __launch_bounds__(LP_WARPS * 32) k_logp(const LogpArgs a) {
   const int64_t lo = first > 0 ? first : 0;
   const int64_t end = first + a.seg;
   const int64_t hi = end < (int64_t)a.cols ? end : (int64_t)a.cols;
+  constexpr int STEP = LP_WARPS * 256;
+  const int64_t mine = first + warp * 256 + lane * 8;  // this thread's vectors: mine + i * STEP
+  if (threadIdx.x == 0) sm.n = 0;
   Stat t = {-INFINITY, 0.0f, 0.0f};
-  TopList best;
-  for (int64_t b = first + warp * 256; b < hi; b += LP_WARPS * 256) {
-    const int64_t e = b + lane * 8;
-    float v[8];
-    load_left<DT>(xr, mr, mask_vec, e, lo, hi, v);
-    stat_add(t, v);
-    if (a.top) {
-      float cm = v[0];
-#pragma unroll
-      for (int j = 1; j < 8; j++) cm = fmaxf(cm, v[j]);
-      // strictly above: a warp sees its elements in ascending order, so an
-      // equal one comes after the one that is listed
-      if (__any_sync(0xffffffffu, cm > best.last_v)) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) best.offer(v[j], (uint32_t)(e + j), a.top, lane);
-      }
+  {
+    int64_t e = mine;
+    for (; e + STEP < hi; e += 2 * STEP) {  // two loads in flight
+      float v[8], u[8];
+      load_left<DT>(xr, mr, mask_vec, e, lo, hi, v);
+      load_left<DT>(xr, mr, mask_vec, e + STEP, lo, hi, u);
+      stat_add(t, v);
+      stat_add(t, u);
+    }
+    if (e < hi) {
+      float v[8];
+      load_left<DT>(xr, mr, mask_vec, e, lo, hi, v);
+      stat_add(t, v);
     }
   }
-  t = warp_stat(t);
-  if (lane == 0) sm_m[warp] = t.m, sm_s[warp] = t.s, sm_w[warp] = t.w;
-  sm_v[warp][lane] = best.v;
-  sm_id[warp][lane] = best.id;
-  __syncthreads();
-  if (warp != 0) return;
-  Stat u = {-INFINITY, 0.0f, 0.0f};
-  if (lane < LP_WARPS) u = {sm_m[lane], sm_s[lane], sm_w[lane]};
-  u = warp_stat(u);
-  if (a.top)
-    for (int w = 1; w < LP_WARPS; w++)
-      best.offer(lane < a.top ? sm_v[w][lane] : -INFINITY, lane < a.top ? sm_id[w][lane] : NO_CHOICE,
-                 a.top, lane);
-  if (a.splits == 1) {
-    finish_row<DT>(a, row, u, best, lane);
-  } else {
-    const uint64_t p = row * a.splits + split;
-    if (lane == 0) a.part[p] = make_float4(u.m, u.s, u.w, 0.0f);
-    if (lane < a.top) {
-      a.part_v[p * a.top + lane] = best.v;
-      a.part_id[p * a.top + lane] = best.id;
+  const uint32_t key = order_key(t.m);
+  t = block_stat(sm, t, warp, lane);
+  const uint64_t p = row * a.splits + split;
+  auto put = [&](int i, float v, uint32_t id) {
+    if (a.splits == 1) {
+      put_top(a, row, t, i, v, id);
+    } else {
+      a.part_v[p * a.top + i] = v;
+      a.part_id[p * a.top + i] = id;
     }
+  };
+  if (a.top) {
+    const uint32_t low = border(key, a.top);
+    // the threads that reach the border, one after the other: the warp reads
+    // four of the thread's vectors at a time
+    uint32_t todo = __ballot_sync(0xffffffffu, key >= low && key != 0);
+    while (todo) {
+      const int src = __ffs((int)todo) - 1;
+      todo &= todo - 1;
+      const int64_t base = first + warp * 256 + src * 8;
+      for (int64_t b = base; b < hi; b += 4 * STEP) {
+        const int64_t e = b + (int64_t)(lane >> 3) * STEP + (lane & 7);
+        const bool in = e >= lo && e < hi && !(mr && mr[e]);
+        const float v = in ? Elt<DT>::get(xr[e]) : -INFINITY;
+        const uint32_t k = order_key(v);
+        add_cands(sm, k >= low && k != 0, v, (uint32_t)e, lane);
+      }
+    }
+    __syncthreads();
+    if (sm.n <= CANDS) {
+      rank_cands(sm, a.top, put);
+    } else {  // hundreds of equal logits: the lists kept while reading
+      TopList best;
+      for (int64_t b = first + warp * 256; b < hi; b += STEP) {
+        const int64_t e = b + lane * 8;
+        float v[8];
+        load_left<DT>(xr, mr, mask_vec, e, lo, hi, v);
+        float cm = v[0];
+#pragma unroll
+        for (int j = 1; j < 8; j++) cm = fmaxf(cm, v[j]);
+        // strictly above: a warp sees its elements in ascending order, so an
+        // equal one comes after the one that is listed
+        if (__any_sync(0xffffffffu, cm > best.last_v)) {
+#pragma unroll
+          for (int j = 0; j < 8; j++) best.offer(v[j], (uint32_t)(e + j), a.top, lane);
+        }
+      }
+      join_lists(sm, best, a.top, warp, lane);
+      if (warp == 0 && lane < a.top) put(lane, best.v, best.id);
+    }
+  }
+  if (threadIdx.x == 0) {
+    if (a.splits == 1) finish_row<DT>(a, row, t);
+    else a.part[p] = make_float4(t.m, t.s, t.w, 0.0f);
   }
 }
 
 // joins a row's segments: one block a row
 template <int DT>
 __global__ void __launch_bounds__(LP_WARPS * 32) k_logp_join(const LogpArgs a) {
-  __shared__ float sm_m[LP_WARPS], sm_s[LP_WARPS], sm_w[LP_WARPS];
-  __shared__ float sm_v[LP_WARPS][TOP_MAX];
-  __shared__ uint32_t sm_id[LP_WARPS][TOP_MAX];
+  __shared__ TopShared sm;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint64_t row = blockIdx.x;
+  if (threadIdx.x == 0) sm.n = 0;
   Stat t = {-INFINITY, 0.0f, 0.0f};
   for (uint32_t s = threadIdx.x; s < a.splits; s += LP_WARPS * 32) {
     const float4 p = a.part[row * a.splits + s];
     t = stat_merge(t, {p.x, p.y, p.z});
   }
-  t = warp_stat(t);
-  TopList best;
+  t = block_stat(sm, t, warp, lane);
   if (a.top) {
     const uint32_t n = a.splits * (uint32_t)a.top;
-    const uint64_t at = row * n;
+    const float* pv = a.part_v + row * n;
+    const uint32_t* pi = a.part_id + row * n;
+    float m = -INFINITY;
+#pragma unroll 8
+    for (uint32_t i = threadIdx.x; i < n; i += LP_WARPS * 32) m = fmaxf(m, pv[i]);
+    const uint32_t low = border(order_key(m), a.top);
     for (uint32_t b = warp * 32; b < n; b += LP_WARPS * 32) {
-      const bool on = b + lane < n;
-      best.offer(on ? a.part_v[at + b + lane] : -INFINITY, on ? a.part_id[at + b + lane] : NO_CHOICE,
-                 a.top, lane);
+      const float v = b + lane < n ? pv[b + lane] : -INFINITY;
+      const uint32_t k = order_key(v);
+      const bool in = k >= low && k != 0;
+      add_cands(sm, in, v, in ? pi[b + lane] : NO_CHOICE, lane);
+    }
+    __syncthreads();
+    if (sm.n <= CANDS) {
+      rank_cands(sm, a.top, [&](int i, float v, uint32_t id) { put_top(a, row, t, i, v, id); });
+    } else {
+      TopList best;
+      for (uint32_t b = warp * 32; b < n; b += LP_WARPS * 32) {
+        const bool on = b + lane < n;
+        best.offer(on ? pv[b + lane] : -INFINITY, on ? pi[b + lane] : NO_CHOICE, a.top, lane);
+      }
+      join_lists(sm, best, a.top, warp, lane);
+      if (warp == 0 && lane < a.top) put_top(a, row, t, lane, best.v, best.id);
     }
   }
-  if (lane == 0) sm_m[warp] = t.m, sm_s[warp] = t.s, sm_w[warp] = t.w;
-  sm_v[warp][lane] = best.v;
-  sm_id[warp][lane] = best.id;
-  __syncthreads();
-  if (warp != 0) return;
-  Stat u = {-INFINITY, 0.0f, 0.0f};
-  if (lane < LP_WARPS) u = {sm_m[lane], sm_s[lane], sm_w[lane]};
-  u = warp_stat(u);
-  if (a.top)
-    for (int w = 1; w < LP_WARPS; w++)
-      best.offer(lane < a.top ? sm_v[w][lane] : -INFINITY, lane < a.top ? sm_id[w][lane] : NO_CHOICE,
-                 a.top, lane);
-  finish_row<DT>(a, row, u, best, lane);
+  if (threadIdx.x == 0) finish_row<DT>(a, row, t);
 }
 
 // short rows: a warp a row
@@ -320,7 +447,9 @@ __global__ void __launch_bounds__(LP_WARPS * 32) k_logp_short(const LogpArgs a) 
         for (int j = 0; j < 8; j++) best.offer(v[j], (uint32_t)(e + j), a.top, lane);
       }
     }
-    finish_row<DT>(a, row, warp_stat(t), best, lane);
+    t = warp_stat(t);
+    if (lane == 0) finish_row<DT>(a, row, t);
+    if (lane < a.top) put_top(a, row, t, lane, best.v, best.id);
   }
 }
 
@@ -393,7 +522,7 @@ __global__ void __launch_bounds__(256) k_logp_bwd(const LogpBwdArgs a) {
       for (int j = 0; j < 8; j++) {
         // what is not left, and all of an empty row, has p = 0 and no gradient
         const float lp = (v[j] - m) - ls;
-        float d = v[j] == -INFINITY ? 0.0f : __expf(lp) * fmaf(-gh, lp, k0);
+        float d = v[j] == -INFINITY ? 0.0f : ex2(lp * LOG2E) * fmaf(-gh, lp, k0);
         if (e + j == (int64_t)c && v[j] != -INFINITY) d += gl;
         v[j] = d;
       }
@@ -435,7 +564,7 @@ int run_logp(bgnn_ctx* ctx, LogpArgs a) {
     BGNN_LAUNCHED(ctx);
     return BGNN_OK;
   }
-  cut_rows(ctx, a.rows, a.cols, 4, 8192, &a.splits, &a.seg);
+  cut_rows(ctx, a.rows, a.cols, 2, 4096, &a.splits, &a.seg);
   DevTmp ws;
   const uint64_t parts = (uint64_t)a.rows * a.splits;
   if (a.splits > 1) {
