@@ -72,8 +72,7 @@ constexpr uint32_t MAX_PER = 512;  // k blocks of a dw range
 
 // One contraction segment: A [m, k] and B [n, k] tiles of one or two tensors.
 // Where `b1` is used (gated), B's tile is rows of b0 above rows of b1.
-// in: the residual or upstream gradient in boxes of a slot, where TMA can take
-// it.
+// in: the residual or upstream gradient in boxes of a slot.
 struct Maps {
   CUtensorMap a[2], b[2], in;
 };
@@ -102,7 +101,6 @@ struct GemmArgs {
   int out_type;
   void* out[2];           // gated backward: dg and du; dw: one a batch
   uint64_t ld_out;
-  int tma_in;             // maps.in is set
   float* part;            // EPI_PARTIAL: [splits, batches, m, ld_out]; NULL: dw whole, no parts
   int* err;
 };
@@ -317,44 +315,13 @@ __device__ __forceinline__ void tmem_wait_ld(float (&v)[32]) {
 }
 
 // ---- activations, f32 ----------------------------------------------------------
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ float rcp(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-constexpr float LOG2E = 1.4426950408889634f;
 // the logistic function 1 / (1 + 2^t), t = -x log2(e)
 __device__ __forceinline__ float sigmoid_t(float t) { return rcp(1.0f + ex2(t)); }
-// two f32 operations in one instruction
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 r;
-  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"
-      " mul.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}\n"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 r;
-  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"
-      " add.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}\n"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"
-      " mov.b64 w, {%6, %7};\n fma.rn.f32x2 z, x, y, w;\n mov.b64 {%0, %1}, z;\n}\n"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 // ... of two arguments.  (One reciprocal for both, 1/a = b/(ab), saves a
 // quarter of the special-function work but costs three more instructions a
@@ -476,40 +443,8 @@ __device__ __forceinline__ void unit16(const uint4 q, int dt, float (&o)[8]) {
     }
   }
 }
-// both slots as 32 rows x 32 f32: where rows cannot go by TMA and are turned
-// round by the warp
-__device__ __forceinline__ float4* turn_unit(void* slots, int row, int unit) {
-  return reinterpret_cast<float4*>(static_cast<char*>(slots) + row * 128 +
-                                   ((unit ^ (row & 7)) << 4));
-}
 __device__ __forceinline__ void fence_async() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
-
-// four consecutive elements along a row, or those of them that exist
-__device__ __forceinline__ float4 load4_row(const void* p, int dt, uint64_t i, uint32_t left,
-                                            bool vec) {
-  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  if (vec && left >= 4) {
-    if (dt == BGNN_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-    const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
-    if (dt == BGNN_BF16)
-      return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u),
-                         __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
-    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-    return make_float4(a.x, a.y, b.x, b.y);
-  }
-  if (left > 0) v.x = load_any(p, dt, i);
-  if (left > 1) v.y = load_any(p, dt, i + 1);
-  if (left > 2) v.z = load_any(p, dt, i + 2);
-  if (left > 3) v.w = load_any(p, dt, i + 3);
-  return v;
-}
-// whether four elements at (row stride ld, column a multiple of 4) are one access
-__device__ __forceinline__ bool vec4_ok(const void* p, int dt, uint64_t ld) {
-  const uint32_t b = dt == BGNN_F32 ? 16u : 8u;
-  return ((uintptr_t)p & (b - 1)) == 0 && ld % 4 == 0;
 }
 
 // whether 16 bytes of a row, from a multiple of as many, are one access
@@ -725,7 +660,6 @@ __global__ void __launch_bounds__(THREADS, 1)
                              ? g.ld_out % 4 == 0
                              : vec16_ok(g.out[0], g.out_type, g.ld_out) &&
                                    (!g.out[1] || vec16_ok(g.out[1], g.out_type, g.ld_out));
-    const bool vec_other = g.other && vec4_ok(g.other, g.other_type, g.ld_other);
     // hands the accumulator back once every lane has read it
     auto release = [&]() {
       tc_fence_before();
@@ -743,7 +677,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // Asks for 32 columns (f32: 16) of the residual / upstream gradient into
       // slot 0, with which every lane is done.
       auto ask = [&](uint32_t col) {
-        if (g.tma_in && lane == 0 && col < g.n) {
+        if (g.other && lane == 0 && col < g.n) {
           fence_async();
           mbar_expect_tx(in_bar, SLOT_BYTES);
           tma_load_2d<1>(s_addr(slots), &maps.in, (int)col, (int)row0, in_bar);
@@ -756,7 +690,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // f(first column, 8 values) for this lane's row of the chunk at col0, eight
       // columns at a time; the first of it was asked for
       auto take = [&](uint32_t col0, auto f) {
-        if (g.tma_in && g.other_type != BGNN_F32) {
+        if (g.other_type != BGNN_F32) {
           asked();
 #pragma unroll
           for (int u = 0; u < 4; u++) {
@@ -765,7 +699,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             f(8 * u, o);
           }
           __syncwarp();
-        } else if (g.tma_in) {
+        } else {
 #pragma unroll
           for (int h = 0; h < 2; h++) {
             if (h == 0 || col0 + 16 < g.n) {
@@ -782,25 +716,6 @@ __global__ void __launch_bounds__(THREADS, 1)
               __syncwarp();
             }
           }
-        } else {  // rows that TMA cannot take: plain reads along rows, turned round
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const int r = i * 4 + (lane >> 3), u = lane & 7;
-            const uint32_t row = row0 + r, col = col0 + u * 4;
-            float4 w = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (row < g.m && col < g.n)
-              w = load4_row(g.other, g.other_type, (uint64_t)row * g.ld_other + col, g.n - col,
-                            vec_other);
-            *turn_unit(slots, r, u) = w;
-          }
-          __syncwarp();
-#pragma unroll
-          for (int u = 0; u < 4; u++) {
-            const float4 a = *turn_unit(slots, lane, 2 * u), b = *turn_unit(slots, lane, 2 * u + 1);
-            const float o[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-            f(8 * u, o);
-          }
-          __syncwarp();
         }
       };
       // Out, a row a lane: through slot 1, turned round, so that four lanes
@@ -1021,22 +936,39 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
-// dw: the splits' partial matrices (rows ld f32 apart) added in order
+// dw: the splits' partial matrices (rows ld f32 apart) added in order: CH chains
+// an element, each in ascending order, then the chains in order.  One chain
+// where elements are many; eight where splits are (47 x 256 over 143 splits:
+// one chain took 14 us, all of it waiting).
+template <int CH>
 __global__ void __launch_bounds__(256) k_add_splits(const float* __restrict__ part, uint32_t splits,
-                                                    uint32_t batches, uint32_t ld,
-                                                    uint32_t rows, uint32_t cols, void* out0,
-                                                    void* out1, int out_type) {
+                                                    uint32_t batches, uint32_t ld, uint32_t rows,
+                                                    uint32_t cols, void* out0, void* out1,
+                                                    int out_type) {
+  constexpr int EL = 256 / CH;
+  __shared__ float sm[CH][EL + 1];
   const uint64_t mn = (uint64_t)rows * cols, total = mn * batches;
   const uint64_t step = (uint64_t)rows * ld * batches;
-  for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-       i += (uint64_t)gridDim.x * blockDim.x) {
+  const int el = threadIdx.x % EL, ch = threadIdx.x / EL;
+  for (uint64_t base = (uint64_t)blockIdx.x * EL; base < total; base += (uint64_t)gridDim.x * EL) {
+    const uint64_t i = base + el;
     const uint32_t b = i >= mn;
     const uint64_t e = b ? i - mn : i;
-    const uint32_t r = (uint32_t)(e / cols), c = (uint32_t)(e - (uint64_t)r * cols);
-    const float* p = part + ((uint64_t)b * rows + r) * ld + c;
-    float v = *p;
-    for (uint32_t s = 1; s < splits; s++) v += p[s * step];
-    store_any(b ? out1 : out0, out_type, e, v);
+    float v = 0.0f;
+    if (i < total) {
+      const uint32_t r = (uint32_t)(e / cols), c = (uint32_t)(e - (uint64_t)r * cols);
+      const float* p = part + ((uint64_t)b * rows + r) * ld + c;
+#pragma unroll 4
+      for (uint32_t s = ch; s < splits; s += CH) v += p[s * step];
+    }
+    if (CH > 1) {
+      sm[ch][el] = v;
+      __syncthreads();
+      if (ch == 0)
+        for (int k = 1; k < CH; k++) v += sm[k][el];
+      __syncthreads();
+    }
+    if (ch == 0 && i < total) store_any(b ? out1 : out0, out_type, e, v);
   }
 }
 
@@ -1141,19 +1073,6 @@ int make_chunk_map(bgnn_ctx* ctx, CUtensorMap* map, int type, const Mat& x) {
     return bgnn_set_error(ctx, BGNN_ERR_UNSUPPORTED, "tensor map encode failed (%d)", (int)r);
   return BGNN_OK;
 }
-// maps.in of a product [m, n] where TMA can take it
-int make_in_map(bgnn_ctx* ctx, Maps* maps, GemmArgs* g) {
-  g->tma_in = 0;
-  if (g->other) {
-    const Mat in = {g->other, g->m, g->n, g->ld_other};
-    if (tma_takes(g->other_type, in)) {
-      BGNN_TRY(make_chunk_map(ctx, &maps->in, g->other_type, in));
-      g->tma_in = 1;
-    }
-  }
-  return BGNN_OK;
-}
-
 // x as TMA can read it: itself, or a copy whose rows start on 16 bytes
 int tma_ready(bgnn_ctx* ctx, int type, Mat* x, DevTmp& tmp) {
   if (tma_takes(type, *x)) return BGNN_OK;
@@ -1164,12 +1083,14 @@ int tma_ready(bgnn_ctx* ctx, int type, Mat* x, DevTmp& tmp) {
   const uint64_t total = x->rows * (uint64_t)ldp, cap = (uint64_t)ctx->num_sms * 16;
   const uint64_t want = (total + 255) / 256;
   const unsigned grid = (unsigned)(want < cap ? want : cap);
-  if (es == 2)
-    k_repack<uint16_t><<<grid, 256, 0, ctx->stream>>>(static_cast<const uint16_t*>(x->p), x->ld,
-                                                       x->rows, x->cols, ldp, tmp.as<uint16_t>());
-  else
-    k_repack<uint8_t><<<grid, 256, 0, ctx->stream>>>(static_cast<const uint8_t*>(x->p), x->ld,
-                                                      x->rows, x->cols, ldp, tmp.as<uint8_t>());
+  auto pack = [&](auto zero) {
+    using T = decltype(zero);
+    k_repack<T><<<grid, 256, 0, ctx->stream>>>(static_cast<const T*>(x->p), x->ld, x->rows, x->cols,
+                                               ldp, tmp.as<T>());
+  };
+  if (es == 4) pack(uint32_t(0));
+  else if (es == 2) pack(uint16_t(0));
+  else pack(uint8_t(0));
   BGNN_LAUNCHED(ctx);
   x->p = tmp.p;
   x->ld = ldp;
@@ -1256,7 +1177,7 @@ int launch(bgnn_ctx* ctx, const Maps& maps, GemmArgs& g, const Shape& s) {
 template <int EPI>
 int run_nt(bgnn_ctx* ctx, GemmArgs& g, Mat x, const Mat (&w)[2], uint32_t k) {
   constexpr bool TWO = EPI == EPI_GATED || EPI == EPI_GATED_BWD;
-  DevTmp tx, tw[2];
+  DevTmp tx, tw[2], tin;
   Maps maps;
   g.a_mn = g.b_mn = 0;
   const Shape sh = pick_shape(ctx, g.m, g.n, 1, TWO, TWO ? 64 : 32);
@@ -1272,7 +1193,11 @@ int run_nt(bgnn_ctx* ctx, GemmArgs& g, Mat x, const Mat (&w)[2], uint32_t k) {
       BGNN_TRY(make_map(ctx, &maps.b[i], g.in_type, wi, TWO ? g.bn / 2 : g.bn / sh.cg));
     }
   }
-  BGNN_TRY(make_in_map(ctx, &maps, &g));
+  if (g.other) {
+    Mat in = {g.other, g.m, g.n, g.ld_other};
+    BGNN_TRY(tma_ready(ctx, g.other_type, &in, tin));
+    BGNN_TRY(make_chunk_map(ctx, &maps.in, g.other_type, in));
+  }
   if constexpr (EPI == EPI_LINEAR)
     if (g.out_type == BGNN_F32) return launch<EPI_LINEAR_F32>(ctx, maps, g, sh);
   return launch<EPI>(ctx, maps, g, sh);
@@ -1350,9 +1275,16 @@ int run_dw(bgnn_ctx* ctx, int type, uint32_t m, uint32_t n, uint32_t k, const Ma
   BGNN_TRY(bgnn_tmp_alloc(ctx, part, (uint64_t)n * g.ld_out * terms * g.splits * sizeof(float)));
   g.part = part.as<float>();
   BGNN_TRY(launch<EPI_PARTIAL>(ctx, maps, g, sh));
-  const uint64_t want = ((uint64_t)n * k * terms + 255) / 256, cap = (uint64_t)ctx->num_sms * 16;
-  k_add_splits<<<(unsigned)(want < cap ? want : cap), 256, 0, ctx->stream>>>(
-      g.part, g.splits, (uint32_t)terms, (uint32_t)g.ld_out, n, k, dw[0], dw[1], type);
+  const int chains = g.splits >= 16 ? 8 : 1;
+  const uint64_t el = 256 / chains;
+  const uint64_t want = ((uint64_t)n * k * terms + el - 1) / el, cap = (uint64_t)ctx->num_sms * 16;
+  const unsigned grid = (unsigned)(want < cap ? want : cap);
+  auto add = [&](auto kernel) {
+    kernel<<<grid, 256, 0, ctx->stream>>>(g.part, g.splits, (uint32_t)terms, (uint32_t)g.ld_out, n,
+                                          k, dw[0], dw[1], type);
+  };
+  if (chains == 8) add(k_add_splits<8>);
+  else add(k_add_splits<1>);
   BGNN_LAUNCHED(ctx);
   return BGNN_OK;
 }
@@ -1492,6 +1424,7 @@ extern "C" int bgnn_linear_fused_backward(bgnn_ctx* ctx, int type, const void* g
   const uint32_t ldz = (n + 7) / 8 * 8;
   Mat dz[2] = {{grad, m, n, ld_grad}, {}};
   DevTmp tz, tg;
+  if (m) BGNN_TRY(tma_ready(ctx, type, &dz[0], tg));  // once for every product that reads it
   if (act != BGNN_ACT_NONE && m) {
     BGNN_TRY(bgnn_tmp_alloc(ctx, tz, m * ldz * 2));
     GemmArgs g = {};
@@ -1502,17 +1435,15 @@ extern "C" int bgnn_linear_fused_backward(bgnn_ctx* ctx, int type, const void* g
     g.bias_type = bias_type;
     g.act = act;
     g.act_p = (float)act_param;
-    g.other = grad;
+    g.other = dz[0].p;
     g.other_type = type;
-    g.ld_other = ld_grad;
+    g.ld_other = dz[0].ld;
     g.out_type = type;
     g.out[0] = tz.p;
     g.ld_out = ldz;
     const Mat ws[2] = {{w, n, k, ld_w}, {w, n, k, ld_w}};
     BGNN_TRY(run_nt<EPI_LINEAR_BWD>(ctx, g, {x, m, k, ld_x}, ws, k));
     dz[0] = {tz.p, m, n, ldz};
-  } else if (m && k && grad_x && grad_w) {
-    BGNN_TRY(tma_ready(ctx, type, &dz[0], tg));  // once for both products
   }
   const Mat ws[2] = {{w, n, k, ld_w}, {}};
   if (grad_x && m && k) BGNN_TRY(run_dx(ctx, type, (uint32_t)m, n, k, dz, ws, 1, grad_x));

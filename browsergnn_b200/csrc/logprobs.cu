@@ -47,20 +47,16 @@ struct LogpArgs {
   int* err;
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LN2 = 0.6931471805599453f;
 // An exponent on its way into 2^a and a 2^a: not below -150, where 2^a is 0, so
 // that a 2^a is never -inf * 0 (x - m may be -inf beside a mask of the type's
 // lowest value).  NaN stays NaN.
-__device__ __forceinline__ float exponent(float d) {
+__device__ __forceinline__ float floored(float a) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(d * LOG2E), "f"(-150.0f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(-150.0f));
   return r;
 }
+__device__ __forceinline__ float exponent(float d) { return floored(d * LOG2E); }
 
 struct Stat {
   float m, s, w;
@@ -152,6 +148,19 @@ __device__ __forceinline__ void load_left(const elt_t<DT>* xr, const uint8_t* mr
   }
 }
 
+// eight elements as they are stored
+template <int DT>
+struct Vec {
+  uint4 w[DT == BGNN_F32 ? 2 : 1];
+};
+template <int DT>
+__device__ __forceinline__ Vec<DT> load_vec(const elt_t<DT>* p) {
+  Vec<DT> r;
+#pragma unroll
+  for (int i = 0; i < (DT == BGNN_F32 ? 2 : 1); i++) r.w[i] = reinterpret_cast<const uint4*>(p)[i];
+  return r;
+}
+
 // elements before the row's first that share its 8-element vector
 template <int DT>
 __device__ __forceinline__ int row_lead(const elt_t<DT>* xr) {
@@ -170,16 +179,18 @@ __device__ __forceinline__ void stat_add(Stat& t, const float (&v)[8]) {
     t.m = cm;
   }
   const float m = t.m == -INFINITY ? 0.0f : t.m;
-  float s0 = 0.0f, s1 = 0.0f;
+  float2 s = make_float2(0.0f, 0.0f), w = make_float2(0.0f, t.w);
+  const float2 mm = make_float2(-m, -m);
 #pragma unroll
   for (int j = 0; j < 8; j += 2) {
-    const float a0 = exponent(v[j] - m), a1 = exponent(v[j + 1] - m);
-    const float e0 = ex2(a0), e1 = ex2(a1);
-    s0 += e0;
-    s1 += e1;
-    t.w = fmaf(a0, e0, fmaf(a1, e1, t.w));
+    const float2 d = mul2(add2(make_float2(v[j], v[j + 1]), mm), make_float2(LOG2E, LOG2E));
+    const float2 a = make_float2(floored(d.x), floored(d.y));
+    const float2 e = make_float2(ex2(a.x), ex2(a.y));
+    s = add2(s, e);
+    w = fma2(a, e, w);
   }
-  t.s += s0 + s1;
+  t.s += s.x + s.y;
+  t.w = w.x + w.y;
 }
 
 // a row's log-sum-exp, entropy and log probability from its statistics
@@ -244,13 +255,14 @@ __device__ __forceinline__ uint32_t border(uint32_t key, int k) {
   return p;
 }
 // appends a candidate a lane; all lanes of the warp call
-__device__ __forceinline__ void add_cands(TopShared& sm, bool in, float v, uint32_t id, int lane) {
+__device__ __forceinline__ void add_cands(float* vs, uint32_t* ids, int* count, int most, bool in,
+                                          float v, uint32_t id, int lane) {
   const uint32_t b = __ballot_sync(0xffffffffu, in);
   if (b == 0) return;
   int at = 0;
-  if (lane == 0) at = atomicAdd(&sm.n, __popc(b));  // their order is not kept: they are ranked
+  if (lane == 0) at = atomicAdd(count, __popc(b));  // their order is not kept: they are ranked
   at = __shfl_sync(0xffffffffu, at, 0) + __popc(b & ((1u << lane) - 1));
-  if (in && at < CANDS) sm.v[at] = v, sm.id[at] = id;
+  if (in && at < most) vs[at] = v, ids[at] = id;
 }
 // the block's statistics, in every thread
 __device__ __forceinline__ Stat block_stat(TopShared& sm, Stat t, int warp, int lane) {
@@ -311,14 +323,30 @@ __global__ void __launch_bounds__(LP_WARPS * 32) k_logp(const LogpArgs a) {
   Stat t = {-INFINITY, 0.0f, 0.0f};
   {
     int64_t e = mine;
-    for (; e + STEP < hi; e += 2 * STEP) {  // two loads in flight
-      float v[8], u[8];
+    if (e < lo) {  // the row starts inside this vector
+      float v[8];
       load_left<DT>(xr, mr, mask_vec, e, lo, hi, v);
-      load_left<DT>(xr, mr, mask_vec, e + STEP, lo, hi, u);
       stat_add(t, v);
-      stat_add(t, u);
+      e += STEP;
     }
-    if (e < hi) {
+    if (!mr) {
+      // whole vectors, four loads in flight
+      const elt_t<DT>* q = xr + e;
+      int64_t left = hi - e;
+      for (; left >= 3 * STEP + 8; left -= 4 * STEP, q += 4 * STEP) {
+        Vec<DT> r[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) r[i] = load_vec<DT>(q + i * STEP);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          float v[8];
+          load8<DT>(reinterpret_cast<const elt_t<DT>*>(r[i].w), v);
+          stat_add(t, v);
+        }
+      }
+      e = hi - left;
+    }
+    for (; e < hi; e += STEP) {
       float v[8];
       load_left<DT>(xr, mr, mask_vec, e, lo, hi, v);
       stat_add(t, v);
@@ -338,18 +366,27 @@ __global__ void __launch_bounds__(LP_WARPS * 32) k_logp(const LogpArgs a) {
   if (a.top) {
     const uint32_t low = border(key, a.top);
     // the threads that reach the border, one after the other: the warp reads
-    // four of the thread's vectors at a time
+    // sixteen of the thread's vectors at a time, four elements a lane
     uint32_t todo = __ballot_sync(0xffffffffu, key >= low && key != 0);
     while (todo) {
       const int src = __ffs((int)todo) - 1;
       todo &= todo - 1;
       const int64_t base = first + warp * 256 + src * 8;
-      for (int64_t b = base; b < hi; b += 4 * STEP) {
+      for (int64_t b = base; b < hi; b += 16 * STEP) {
+        float v[4];
         const int64_t e = b + (int64_t)(lane >> 3) * STEP + (lane & 7);
-        const bool in = e >= lo && e < hi && !(mr && mr[e]);
-        const float v = in ? Elt<DT>::get(xr[e]) : -INFINITY;
-        const uint32_t k = order_key(v);
-        add_cands(sm, k >= low && k != 0, v, (uint32_t)e, lane);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int64_t q = e + i * (4 * STEP);
+          const bool in = q >= lo && q < hi && !(mr && mr[q]);
+          v[i] = in ? Elt<DT>::get(xr[q]) : -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const uint32_t k = order_key(v[i]);
+          add_cands(sm.v, sm.id, &sm.n, CANDS, k >= low && k != 0, v[i],
+                    (uint32_t)(e + i * (4 * STEP)), lane);
+        }
       }
     }
     __syncthreads();
@@ -406,7 +443,7 @@ __global__ void __launch_bounds__(LP_WARPS * 32) k_logp_join(const LogpArgs a) {
       const float v = b + lane < n ? pv[b + lane] : -INFINITY;
       const uint32_t k = order_key(v);
       const bool in = k >= low && k != 0;
-      add_cands(sm, in, v, in ? pi[b + lane] : NO_CHOICE, lane);
+      add_cands(sm.v, sm.id, &sm.n, CANDS, in, v, in ? pi[b + lane] : NO_CHOICE, lane);
     }
     __syncthreads();
     if (sm.n <= CANDS) {
@@ -424,32 +461,82 @@ __global__ void __launch_bounds__(LP_WARPS * 32) k_logp_join(const LogpArgs a) {
   if (threadIdx.x == 0) finish_row<DT>(a, row, t);
 }
 
-// short rows: a warp a row
-template <int DT>
+// Short rows: a warp a row, the whole row in its registers (E elements a lane,
+// element i of lane l being i * 32 + l), so the maximum comes first and nothing
+// is rescaled.  The list as in k_logp, its border from the 32 lane maxima.
+constexpr int SHORT_CANDS = 64;
+template <int DT, int E>
 __global__ void __launch_bounds__(LP_WARPS * 32) k_logp_short(const LogpArgs a) {
-  const int lane = threadIdx.x & 31;
+  __shared__ float sm_v[LP_WARPS][SHORT_CANDS];
+  __shared__ uint32_t sm_id[LP_WARPS][SHORT_CANDS];
+  __shared__ int sm_n[LP_WARPS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint64_t step = (uint64_t)gridDim.x * LP_WARPS;
-  for (uint64_t row = (uint64_t)blockIdx.x * LP_WARPS + (threadIdx.x >> 5); row < a.rows;
-       row += step) {
+  for (uint64_t row = (uint64_t)blockIdx.x * LP_WARPS + warp; row < a.rows; row += step) {
     const elt_t<DT>* xr = static_cast<const elt_t<DT>*>(a.x) + row * a.ld;
     const uint8_t* mr = a.mask ? a.mask + row * a.ld_mask : nullptr;
-    const int64_t lead = row_lead<DT>(xr), hi = a.cols;
-    const bool mask_vec = mr && (((uintptr_t)mr - (uintptr_t)lead) & 7u) == 0;
-    Stat t = {-INFINITY, 0.0f, 0.0f};
-    TopList best;
-    for (int64_t b = -lead; b < hi; b += 256) {
-      const int64_t e = b + lane * 8;
-      float v[8];
-      load_left<DT>(xr, mr, mask_vec, e, 0, hi, v);
-      stat_add(t, v);
-      if (a.top) {
+    float v[E];
+    float m = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 8; j++) best.offer(v[j], (uint32_t)(e + j), a.top, lane);
-      }
+    for (int i = 0; i < E; i++) {
+      const uint32_t c = i * 32 + lane;
+      v[i] = c < a.cols && !(mr && mr[c]) ? Elt<DT>::get(xr[c]) : -INFINITY;
+      m = fmaxf(m, v[i]);
     }
-    t = warp_stat(t);
+    const uint32_t key = order_key(m);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float ms = m == -INFINITY ? 0.0f : m;
+    Stat t = {m, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < E; i++) {
+      const float q = exponent(v[i] - ms), e = ex2(q);
+      t.s += e;
+      t.w = fmaf(q, e, t.w);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      t.s += __shfl_xor_sync(0xffffffffu, t.s, o);
+      t.w += __shfl_xor_sync(0xffffffffu, t.w, o);
+    }
     if (lane == 0) finish_row<DT>(a, row, t);
-    if (lane < a.top) put_top(a, row, t, lane, best.v, best.id);
+    if (a.top) {
+      uint32_t low = 0;
+      for (int bit = 31; bit >= 0; bit--) {
+        const uint32_t q = low | (1u << bit);
+        const int c = __popc(__ballot_sync(0xffffffffu, key >= q));
+        if (c >= a.top) {
+          low = q;
+          if (c <= a.top + 4) break;
+        }
+      }
+      if (lane == 0) sm_n[warp] = 0;
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < E; i++) {
+        const uint32_t k = order_key(v[i]);
+        add_cands(sm_v[warp], sm_id[warp], &sm_n[warp], SHORT_CANDS, k >= low && k != 0, v[i],
+                  i * 32 + lane, lane);
+      }
+      __syncwarp();
+      const int n = sm_n[warp];
+      if (n <= SHORT_CANDS) {
+        for (int i = lane; i < n; i += 32) {
+          const float cv = sm_v[warp][i];
+          const uint32_t ci = sm_id[warp][i];
+          int r = 0;
+          for (int j = 0; j < n; j++) r += before(sm_v[warp][j], sm_id[warp][j], cv, ci);
+          if (r < a.top) put_top(a, row, t, r, cv, ci);
+        }
+        if (lane >= n && lane < a.top) put_top(a, row, t, lane, -INFINITY, NO_CHOICE);
+      } else {
+        TopList best;
+#pragma unroll
+        for (int i = 0; i < E; i++) best.offer(v[i], i * 32 + lane, a.top, lane);
+        if (lane < a.top) put_top(a, row, t, lane, best.v, best.id);
+      }
+      __syncwarp();
+    }
   }
 }
 
@@ -473,8 +560,47 @@ struct LogpBwdArgs {
 // such a row's m and log S are summed again by every block that works on it.
 constexpr float LSE_EXACT = 128.0f;
 
+// an element's gradient; x -inf: not left, and all of an empty row: none
+__device__ __forceinline__ float grad_of(float x, float m, float ls, float k0, float gl, float gh,
+                                         bool hit) {
+  const float lp = (x - m) - ls;
+  const float d = ex2(lp * LOG2E) * fmaf(-gh, lp, k0);
+  return x == -INFINITY ? 0.0f : hit ? d + gl : d;
+}
+
+// short rows: a warp a row, an element a lane at a time
 template <int DT>
-__global__ void __launch_bounds__(256) k_logp_bwd(const LogpBwdArgs a) {
+__global__ void __launch_bounds__(256) k_logp_bwd_short(const LogpBwdArgs a) {
+  const int lane = threadIdx.x & 31;
+  const uint64_t step = (uint64_t)gridDim.x * 8;
+  for (uint64_t row = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < a.rows; row += step) {
+    const elt_t<DT>* xr = static_cast<const elt_t<DT>*>(a.x) + row * a.ld;
+    elt_t<DT>* dr = static_cast<elt_t<DT>*>(a.dx) + row * a.cols;
+    const uint8_t* mr = a.mask ? a.mask + row * a.ld_mask : nullptr;
+    const uint32_t c = a.targets[row];
+    if (c != NO_CHOICE && c >= a.cols && lane == 0) dev_raise(a.err, DEVERR_INDEX, c, 61);
+    const float gl = a.g_logp && c != NO_CHOICE ? a.g_logp[row] : 0.0f;
+    const float gh = a.g_ent ? a.g_ent[row] : 0.0f;
+    const float k0 = fmaf(-gh, a.g_ent ? a.entropy[row] : 0.0f, -gl);
+    float m = 0.0f, ls = a.lse[row];
+    auto at = [&](uint32_t e) {
+      return mr && mr[e] ? -INFINITY : Elt<DT>::get(xr[e]);
+    };
+    if (fabsf(ls) >= LSE_EXACT && fabsf(ls) < INFINITY) {
+      Stat t = {-INFINITY, 0.0f, 0.0f};
+      for (uint32_t e = lane; e < a.cols; e += 32) t = stat_merge(t, {at(e), 1.0f, 0.0f});
+      t = warp_stat(t);
+      m = t.m;
+      ls = logf(t.s);
+    }
+#pragma unroll 4
+    for (uint32_t e = lane; e < a.cols; e += 32)
+      dr[e] = Elt<DT>::put(grad_of(at(e), m, ls, k0, gl, gh, e == c));
+  }
+}
+
+template <int DT>
+__global__ void __launch_bounds__(256, 8) k_logp_bwd(const LogpBwdArgs a) {
   __shared__ float sm_m[8], sm_s[8];
   const uint64_t units = (uint64_t)a.rows * a.splits;
   for (uint64_t u = blockIdx.x; u < units; u += gridDim.x) {
@@ -519,13 +645,8 @@ __global__ void __launch_bounds__(256) k_logp_bwd(const LogpBwdArgs a) {
       float v[8];
       load_left<DT>(xr, mr, mask_vec, e, lo, hi, v);
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        // what is not left, and all of an empty row, has p = 0 and no gradient
-        const float lp = (v[j] - m) - ls;
-        float d = v[j] == -INFINITY ? 0.0f : ex2(lp * LOG2E) * fmaf(-gh, lp, k0);
-        if (e + j == (int64_t)c && v[j] != -INFINITY) d += gl;
-        v[j] = d;
-      }
+      for (int j = 0; j < 8; j++)
+        v[j] = grad_of(v[j], m, ls, k0, gl, gh, e + j == (int64_t)c);
       if (out_vec && e >= lo && e + 8 <= hi) {
         store8<DT>(dr + e, v);
       } else {
@@ -560,7 +681,11 @@ int run_logp(bgnn_ctx* ctx, LogpArgs a) {
   if (a.cols <= LP_SHORT) {
     const uint64_t want = ((uint64_t)a.rows + LP_WARPS - 1) / LP_WARPS;
     const uint64_t cap = (uint64_t)ctx->num_sms * 8;
-    k_logp_short<DT><<<(unsigned)(want < cap ? want : cap), LP_WARPS * 32, 0, ctx->stream>>>(a);
+    const unsigned grid = (unsigned)(want < cap ? want : cap);
+    if (a.cols <= 64) k_logp_short<DT, 2><<<grid, LP_WARPS * 32, 0, ctx->stream>>>(a);
+    else if (a.cols <= 256) k_logp_short<DT, 8><<<grid, LP_WARPS * 32, 0, ctx->stream>>>(a);
+    else if (a.cols <= 512) k_logp_short<DT, 16><<<grid, LP_WARPS * 32, 0, ctx->stream>>>(a);
+    else k_logp_short<DT, 32><<<grid, LP_WARPS * 32, 0, ctx->stream>>>(a);
     BGNN_LAUNCHED(ctx);
     return BGNN_OK;
   }
@@ -584,6 +709,12 @@ int run_logp(bgnn_ctx* ctx, LogpArgs a) {
 
 template <int DT>
 int run_logp_bwd(bgnn_ctx* ctx, LogpBwdArgs a) {
+  if (a.cols <= LP_SHORT) {
+    const uint64_t want = ((uint64_t)a.rows + 7) / 8, cap = (uint64_t)ctx->num_sms * 16;
+    k_logp_bwd_short<DT><<<(unsigned)(want < cap ? want : cap), 256, 0, ctx->stream>>>(a);
+    BGNN_LAUNCHED(ctx);
+    return BGNN_OK;
+  }
   cut_rows(ctx, a.rows, a.cols, 8, 2048, &a.splits, &a.seg);
   const uint64_t units = (uint64_t)a.rows * a.splits, cap = (uint64_t)ctx->num_sms * 64;
   k_logp_bwd<DT><<<(unsigned)(units < cap ? units : cap), 256, 0, ctx->stream>>>(a);

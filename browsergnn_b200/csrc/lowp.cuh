@@ -152,3 +152,37 @@ __device__ __forceinline__ void store_any(void* p, int dt, uint64_t i, float v) 
   else if (dt == BGNN_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
   else static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
+
+// ---- f32 arithmetic that the kernels share ---------------------------------------
+constexpr float LOG2E = 1.4426950408889634f;
+// 2^x, two units in the last place; results below the normal range are 0
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// two f32 operations in one instruction
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"
+      " mul.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"
+      " add.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"
+      " mov.b64 w, {%6, %7};\n fma.rn.f32x2 z, x, y, w;\n mov.b64 {%0, %1}, z;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
