@@ -43,8 +43,8 @@ class CudaContext:
         self._math = _lib.MATH_FAST
 
     def bind(self):
-        torch = _torch()
-        s = torch.cuda.current_stream(self.device).cuda_stream
+        # current_stream(device).cuda_stream without building a Stream object
+        s = _torch()._C._cuda_getCurrentRawStream(self.device)
         if s != self._stream:
             _lib.check(self.lib.bgnn_ctx_set_stream(self.h, s if s else None), self.h)
             self._stream = s

@@ -40,15 +40,29 @@ def _torch():
     return torch
 
 
+_TENSOR = ()  # (torch.Tensor,), filled on first use
+
+
+def _tensor_class():
+    global _TENSOR
+    _TENSOR = (_torch().Tensor,)
+    return _TENSOR
+
+
+_CODES = {}  # torch dtype -> bgnn_dtype, filled on first use
+
+
 def _codes():
-    torch = _torch()
-    return {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16,
-            torch.float8_e4m3fn: _lib.E4M3}
+    if not _CODES:
+        torch = _torch()
+        _CODES.update({torch.float32: _lib.F32, torch.bfloat16: _lib.BF16,
+                       torch.float16: _lib.F16, torch.float8_e4m3fn: _lib.E4M3})
+    return _CODES
 
 
 def _type(dtype, name, allowed):
     """bgnn_dtype of a torch dtype, one of `allowed`."""
-    code = _codes().get(dtype)
+    code = (_CODES or _codes()).get(dtype)
     if code not in allowed:
         names = {v: str(k).replace("torch.", "") for k, v in _codes().items()}
         raise TypeError(f"{name} has type {dtype}; "
@@ -61,7 +75,7 @@ _HALVES = (_lib.BF16, _lib.F16)
 
 
 def _tensor(t, name):
-    if not isinstance(t, _torch().Tensor):
+    if not isinstance(t, (_TENSOR or _tensor_class())):
         raise TypeError(f"{name} must be a CUDA tensor")
     return t
 
@@ -73,12 +87,13 @@ def _device(**tensors):
     for name, t in tensors.items():
         if t is None:
             continue
-        if not t.is_cuda:
+        d = t.get_device()  # -1: not on a GPU
+        if d < 0:
             raise TypeError(f"{name} must be a CUDA tensor")
-        if dev is not None and t.device.index != dev:
-            raise ValueError(f"{name} is on cuda:{t.device.index}, the other operands on "
-                             f"cuda:{dev}")
-        dev = t.device.index
+        if dev is None:
+            dev = d
+        elif d != dev:
+            raise ValueError(f"{name} is on cuda:{d}, the other operands on cuda:{dev}")
     return dev
 
 
@@ -86,13 +101,15 @@ def _rows(t, name):
     """[rows, cols] with unit column stride and rows that do not overlap, and
     whether the tensor was one row."""
     _tensor(t, name)
-    if t.dim() not in (1, 2):
-        raise ValueError(f"{name}: expects 1D or 2D input, got {t.dim()}D")
     one = t.dim() == 1
     if one:
         t = t.unsqueeze(0)
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        t = t.contiguous()
+    elif t.dim() != 2:
+        raise ValueError(f"{name}: expects 1D or 2D input, got {t.dim()}D")
+    if not t.is_contiguous():
+        rows, cols = t.shape
+        if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+            t = t.contiguous()
     if t.shape[1] >= 2 ** 31:
         raise ValueError(f"{name}: a row of {t.shape[1]} elements")
     return t, one
@@ -100,7 +117,8 @@ def _rows(t, name):
 
 def _ld(t):
     """Row stride in elements (a single row's is its length)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    rows, cols = t.shape
+    return t.stride(0) if rows > 1 else cols
 
 
 def _vec(t, n, name, allowed):
@@ -127,7 +145,7 @@ def _act(act):
 
 
 def _empty(shape, dtype, like):
-    return _torch().empty(shape, dtype=dtype, device=like.device)
+    return like.new_empty(shape, dtype=dtype)
 
 
 # ---------------------------------------------------------------------------

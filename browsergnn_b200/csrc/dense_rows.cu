@@ -1,0 +1,173 @@
+// The products of dense16.cu for a few rows of x (one token or node served, or
+// a handful): out = act(x w^T + b) + residual and
+// out = act(x wg^T + bg) * (x wu^T + bu).
+//
+// Bound by the weights' bytes: each weight is read once and used m times, far
+// below what would feed the tensor cores.  A warp owns one output column: its
+// lanes stream the weight's row (rows) in 16-byte pieces, several in flight,
+// multiply with the rows of x (which stay in L1), and add up in f32: one chain
+// a lane, then a tree of shuffles.  Rows that do not start on 16 bytes are read
+// an element a lane.
+#include "lowp.cuh"
+
+#include "dense_rows.cuh"
+
+namespace {
+
+constexpr int WARPS = 8;
+
+// the elements of one 16-byte piece, or one element
+template <int DT, int VEC>
+__device__ __forceinline__ void piece(const void* row, uint32_t c, float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    if constexpr (DT == BGNN_E4M3)
+      v[0] = __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t*>(row)[c],
+                                                         __NV_E4M3)));
+    else
+      v[0] = Elt<DT>::get(static_cast<const elt_t<DT>*>(row)[c]);
+  } else if constexpr (DT == BGNN_E4M3) {
+    const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(row) + c);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(
+          (__nv_fp8x2_storage_t)(w[i >> 1] >> (16 * (i & 1))), __NV_E4M3);
+      const float2 f = __half22float2(__half2(h));
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  } else {
+    load8<DT>(static_cast<const elt_t<DT>*>(row) + c, v);
+  }
+}
+
+template <int DT, int M, bool TWO, int VEC>
+__global__ void __launch_bounds__(WARPS * 32) k_dense_rows(const RowsArgs a) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t col = blockIdx.x * WARPS + (threadIdx.x >> 5);
+  if (col >= a.n) return;
+  constexpr uint32_t ES = DT == BGNN_E4M3 ? 1 : 2;
+  const char* w[2];
+  w[0] = static_cast<const char*>(a.w[0]) + (uint64_t)col * a.ld_w[0] * ES;
+  w[1] = TWO ? static_cast<const char*>(a.w[1]) + (uint64_t)col * a.ld_w[1] * ES : nullptr;
+  const char* x[M];
+#pragma unroll
+  for (int i = 0; i < M; i++)  // a row that is not there repeats the last
+    x[i] = static_cast<const char*>(a.x) +
+           (uint64_t)(i < (int)a.m ? i : (int)a.m - 1) * a.ld_x * ES;
+  float s[TWO ? 2 : 1][M];
+#pragma unroll
+  for (int t = 0; t < (TWO ? 2 : 1); t++)
+#pragma unroll
+    for (int i = 0; i < M; i++) s[t][i] = 0.0f;
+  auto add = [&](const float (&u)[VEC], const float (&g)[VEC], uint32_t c) {
+#pragma unroll
+    for (int i = 0; i < M; i++) {
+      float v[VEC];
+      piece<DT, VEC>(x[i], c, v);
+#pragma unroll
+      for (int j = 0; j < VEC; j++) {
+        s[0][i] = fmaf(u[j], v[j], s[0][i]);
+        if (TWO) s[TWO][i] = fmaf(g[j], v[j], s[TWO][i]);
+      }
+    }
+  };
+  constexpr uint32_t STEP = 32 * VEC;
+  constexpr int DEEP = VEC == 1 ? 8 : 4;  // pieces in flight
+  uint32_t c = lane * VEC;
+  for (; c + (DEEP - 1) * STEP + VEC <= a.k; c += DEEP * STEP) {
+    float u[DEEP][VEC], g[DEEP][VEC];
+#pragma unroll
+    for (int d = 0; d < DEEP; d++) {
+      piece<DT, VEC>(w[0], c + d * STEP, u[d]);
+      if (TWO) piece<DT, VEC>(w[1], c + d * STEP, g[d]);
+    }
+#pragma unroll
+    for (int d = 0; d < DEEP; d++) add(u[d], g[d], c + d * STEP);
+  }
+  for (; c + VEC <= a.k; c += STEP) {
+    float u[VEC], g[VEC];
+    piece<DT, VEC>(w[0], c, u);
+    if (TWO) piece<DT, VEC>(w[1], c, g);
+    add(u, g, c);
+  }
+  if (VEC > 1) {  // the last columns, fewer than a piece: an element a lane
+    const uint32_t e = a.k / VEC * VEC + lane;
+    if (e < a.k) {
+      float u[1], g[1] = {0.0f}, v[1];
+      piece<DT, 1>(w[0], e, u);
+      if (TWO) piece<DT, 1>(w[1], e, g);
+#pragma unroll
+      for (int i = 0; i < M; i++) {
+        piece<DT, 1>(x[i], e, v);
+        s[0][i] = fmaf(u[0], v[0], s[0][i]);
+        if (TWO) s[TWO][i] = fmaf(g[0], v[0], s[TWO][i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int t = 0; t < (TWO ? 2 : 1); t++)
+#pragma unroll
+      for (int i = 0; i < M; i++) s[t][i] += __shfl_xor_sync(0xffffffffu, s[t][i], o);
+  // lane i finishes row i
+  float z0 = 0.0f, z1 = 0.0f;
+#pragma unroll
+  for (int i = 0; i < M; i++)
+    if (lane == i) {
+      z0 = s[0][i];
+      if (TWO) z1 = s[TWO][i];
+    }
+  if (lane >= (int)a.m) return;
+  if (DT == BGNN_E4M3) {
+    z0 *= a.x_scale[lane] * a.w_scale[0][col];
+    if (TWO) z1 *= a.x_scale[lane] * a.w_scale[1][col];
+  }
+  if (a.bias[0]) z0 += load_any(a.bias[0], a.bias_type, col);
+  if (TWO && a.bias[1]) z1 += load_any(a.bias[1], a.bias_type, col);
+  float o = z0;
+  with_act(a.act, [&](auto act) {
+    o = act_two<decltype(act)::value>(make_float2(z0, 0.0f), a.act_p).x;
+  });
+  if (TWO) o *= z1;
+  else if (a.other) o += load_any(a.other, a.other_type, (uint64_t)lane * a.ld_other + col);
+  store_any(a.out, a.out_type, (uint64_t)lane * a.ld_out + col, o);
+}
+
+template <int DT, int M, bool TWO>
+int launch_vec(bgnn_ctx* ctx, const RowsArgs& a, bool vec) {
+  const unsigned grid = (a.n + WARPS - 1) / WARPS;
+  constexpr int VEC = DT == BGNN_E4M3 ? 16 : 8;
+  if (vec) k_dense_rows<DT, M, TWO, VEC><<<grid, WARPS * 32, 0, ctx->stream>>>(a);
+  else k_dense_rows<DT, M, TWO, 1><<<grid, WARPS * 32, 0, ctx->stream>>>(a);
+  BGNN_LAUNCHED(ctx);
+  return BGNN_OK;
+}
+template <int DT, bool TWO>
+int launch_m(bgnn_ctx* ctx, const RowsArgs& a, bool vec) {
+  if (a.m == 1) return launch_vec<DT, 1, TWO>(ctx, a, vec);
+  if (a.m == 2) return launch_vec<DT, 2, TWO>(ctx, a, vec);
+  if (a.m <= 4) return launch_vec<DT, 4, TWO>(ctx, a, vec);
+  return launch_vec<DT, 8, TWO>(ctx, a, vec);
+}
+template <int DT>
+int launch_two(bgnn_ctx* ctx, const RowsArgs& a, bool vec) {
+  return a.two ? launch_m<DT, true>(ctx, a, vec) : launch_m<DT, false>(ctx, a, vec);
+}
+
+}  // namespace
+
+int bgnn_run_dense_rows(bgnn_ctx* ctx, int type, const RowsArgs& a) {
+  const uint32_t es = (uint32_t)dtype_size(type);
+  auto whole = [&](const void* p, uint64_t ld) {
+    return ((uintptr_t)p & 15u) == 0 && ld * es % 16 == 0;
+  };
+  const bool vec = whole(a.x, a.ld_x) && whole(a.w[0], a.ld_w[0]) &&
+                   (!a.two || whole(a.w[1], a.ld_w[1]));
+  switch (type) {
+    case BGNN_BF16: return launch_two<BGNN_BF16>(ctx, a, vec);
+    case BGNN_F16: return launch_two<BGNN_F16>(ctx, a, vec);
+    default: return launch_two<BGNN_E4M3>(ctx, a, vec);
+  }
+}

@@ -221,6 +221,11 @@ PRODUCTS = [  # m, k, n, type, act, bias, residual, out
     (200, 160, 96, F8, "gelu", BF, BF, BF), (129, 1040, 300, F8, None, None, F32, F32),
     (40, 250, 33, F8, "silu", None, None, BF), (20000, 64, 640, BF, "relu", BF, None, BF),
     (2, 1, 1, F16, None, None, None, F32), (9, 0, 20, BF, "silu", BF, F32, F32),
+    # few rows, and the first past them
+    (2, 1040, 70, F8, "gelu", BF, F32, BF), (4, 2050, 33, BF, "relu", F32, BF, F32),
+    (3, 75, 130, F8, None, None, None, F32), (4, 0, 9, F16, "sigmoid", F16, None, F16),
+    (5, 2050, 33, BF, "relu", F32, BF, F32), (1, 4096, 4100, BF, "silu", None, None, BF),
+    (8, 300, 64, F16, "tanh", None, F16, F16), (9, 300, 64, F16, "tanh", None, F16, F16),
 ]
 
 
@@ -252,7 +257,9 @@ def test_linear_fused(m, k, n, t, act, tb, tr, to, how):
     (257, 256, 513, F16, "sigmoid", None), (40, 250, 33, BF, None, BF),
     (64, 1433, 160, BF, "relu", None), (300, 160, 96, F8, "silu", BF), (129, 1040, 300, F8, "gelu",
                                                                         None),
-    (20000, 64, 320, BF, "tanh", None), (3, 5, 7, F16, ("elu", 1.0), None), (4, 0, 9, BF, "silu", BF)])
+    (20000, 64, 320, BF, "tanh", None), (3, 5, 7, F16, ("elu", 1.0), None), (4, 0, 9, BF, "silu", BF),
+    (1, 1040, 70, F8, "gelu", BF), (2, 300, 40, F8, "silu", None), (4, 2050, 33, F16, "relu", F32),
+    (5, 2050, 33, F16, "relu", F32), (8, 1040, 70, F8, "gelu", BF), (9, 1040, 70, F8, "gelu", BF)])
 def test_gated_linear(m, k, n, t, act, tb, how):
     g = gen(m + 3 * k + 5 * n)
     std = math.sqrt(2 / (k + n))
