@@ -29,8 +29,8 @@ from .layers import (ELU, GATConv, GCNConv, GINConv, LeakyReLU, Module, ReLU, SA
                      Sequential, global_sum_pool)
 from .ops import (GPUSparse, GPUTensor, MessagePassing, SparseCOO, SparseCSR, compute_gcn_norm,
                   computeGCNNorm)
-from .nn import (GELU, Dropout, Linear, LogSoftmax, PReLU, SiLU, Sigmoid, Softmax, Tanh,
-                 manual_seed)
+from .nn import (GELU, Dropout, GatedFeedForward, Linear, LogSoftmax, PReLU, RMSNorm, SiLU, Sigmoid,
+                 Softmax, Tanh, manual_seed)
 from .models import ConceptPrerequisiteMapper, LearningPathRecommender, StudentMasteryPredictor
 from . import blocks, serialization
 from .blocks import (gated_linear, gated_linear_backward, gatedLinear, gatedLinearBackward,
@@ -53,5 +53,5 @@ __all__ = [
     "manual_seed", "StudentMasteryPredictor", "LearningPathRecommender",
     "ConceptPrerequisiteMapper", "serialization", "serializeModel", "deserializeModel",
     "saveModelToJSON", "loadModelFromJSON", "getStateDict", "loadStateDict", "getModelSize",
-    "CapturedForward", *blocks.__all__, "blocks",
+    "CapturedForward", "RMSNorm", "GatedFeedForward", *blocks.__all__, "blocks",
 ]

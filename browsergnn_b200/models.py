@@ -23,6 +23,7 @@ import numpy as np
 
 from . import _lib
 from .backend import get_context, ptr
+from .blocks import logProbs
 from .graph import GraphData
 from .layers import GATConv, GCNConv, GINConv, Module, SAGEConv, _param, _torch, next_dropout_seed
 from .nn import ELU, Dropout, LeakyReLU, Linear, ReLU, Sequential, Sigmoid, Softmax
@@ -194,9 +195,9 @@ class LearningPathRecommender(Module):
         self.registerModule("scoringHead", self.scoringHead)
         self.softmax = Softmax()
 
-    def forward(self, graph: GraphData, maskMastered: Optional[Sequence[bool]] = None):
-        """[numNodes, 1] scores (LearningPathRecommender.ts:173-225)."""
-        torch = _torch()
+    def _scores(self, graph: GraphData):
+        """[numNodes, 1] scores before mask and softmax
+        (LearningPathRecommender.ts:173-189)."""
         h = self.inputProj.forward(graph.x_device())
         wg = graph.withFeatures(h)
         n_layers = len(self.gnnLayers)
@@ -206,7 +207,12 @@ class LearningPathRecommender(Module):
                 wg = wg.withFeatures(_dropout(self.dropout, wg.x))
             else:
                 wg = layer.forward(wg)
-        scores = self.scoringHead.forward(wg.x).contiguous()
+        return self.scoringHead.forward(wg.x).contiguous()
+
+    def forward(self, graph: GraphData, maskMastered: Optional[Sequence[bool]] = None):
+        """[numNodes, 1] scores (LearningPathRecommender.ts:173-225)."""
+        torch = _torch()
+        scores = self._scores(graph)
         n = graph.numNodes
         mask_t = None
         if maskMastered is not None:
@@ -237,6 +243,31 @@ class LearningPathRecommender(Module):
         scored.sort(key=lambda p: -p["score"])
         recs = [dict(p, rank=r + 1) for r, p in enumerate(scored[:topK])]
         return {"recommendations": recs, "allScores": all_scores}
+
+    def stepLogProb(self, graph: GraphData, chosenNode: int, masteredNodes: Sequence[int] = (),
+                    topK: int = 5):
+        """How likely the model finds ``chosenNode`` as the next step: its log
+        probability among the nodes not yet mastered, the entropy of that
+        choice, and the topK alternatives (eval mode; no counterpart in the
+        reference).  A mastered node has probability zero; equal scores come
+        in ascending node order, as in recommend."""
+        torch = _torch()
+        if not 0 <= int(chosenNode) < graph.numNodes:
+            raise ValueError(f"chosenNode {chosenNode} out of bounds for {graph.numNodes} nodes")
+        self.eval()
+        scores = self._scores(graph).reshape(1, -1)
+        m = np.zeros(graph.numNodes, np.uint8)
+        m[[int(i) for i in masteredNodes]] = 1
+        mask = torch.from_numpy(m).to(scores.device)
+        target = torch.tensor([int(chosenNode)], dtype=torch.int32, device=scores.device)
+        logp, entropy, _, ids, top = logProbs(scores, target, mask=mask, topK=int(topK))
+        alternatives = []
+        if topK:
+            alternatives = [{"nodeIndex": i, "logProb": v, "rank": r + 1}
+                            for r, (i, v) in enumerate(zip(ids[0].tolist(), top[0].tolist()))
+                            if i >= 0]
+        return {"logProb": float(logp[0]), "entropy": float(entropy[0]),
+                "alternatives": alternatives}
 
     def getLearningPath(self, graph: GraphData, masteredNodes: Sequence[int],
                         goalNodes: Sequence[int], maxSteps: int = 20):

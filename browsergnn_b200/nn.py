@@ -5,7 +5,8 @@ Linear (src/nn/linear.ts), the activation modules of src/nn/activation.ts
 Dropout) and the Module / Sequential containers of src/nn/module.ts.  Same
 constructor arguments, parameter names and shapes, defaults and errors as the
 reference; ``forward`` takes a CUDA tensor (or a GraphData, whose features it
-transforms) and returns the same kind.
+transforms) and returns the same kind.  RMSNorm and GatedFeedForward are this
+backend's own, over the mixed-precision operators of blocks.py.
 
 Training-mode Dropout draws from a counter-based generator (libbgnn_cuda's
 bgnn_dropout) instead of Math.random(): the keep/scale rule is the
@@ -20,13 +21,16 @@ import numpy as np
 
 from . import _lib
 from .backend import get_context, ptr
+from .blocks import (gatedLinear, gatedLinearBackward, linearFused, linearFusedBackward, rmsNorm,
+                     rmsNormBackward)
 from .graph import GraphData
 from .layers import (ELU, LeakyReLU, Module, ReLU, Sequential, _Act, _param, _torch,
                      manual_seed, next_dropout_seed, register_fusable)
 
 __all__ = [
     "Module", "Sequential", "Linear", "ReLU", "LeakyReLU", "ELU", "Sigmoid", "Tanh", "GELU",
-    "SiLU", "PReLU", "Softmax", "LogSoftmax", "Dropout", "manual_seed",
+    "SiLU", "PReLU", "Softmax", "LogSoftmax", "Dropout", "RMSNorm", "GatedFeedForward",
+    "manual_seed",
 ]
 
 
@@ -177,6 +181,123 @@ class Dropout(Module):
         s = next_dropout_seed() if seed is None else int(seed)
         get_context(x.device.index).call("bgnn_dropout", ptr(x), x.numel(), self.p, s, ptr(out))
         return _wrap(input, out)
+
+
+def _tensor_on_device(module, input):
+    """The f32 CUDA rows of a tensor or a GraphData, the module moved to them."""
+    torch = _torch()
+    x = _tensor_of(input)
+    if not hasattr(x, "is_cuda"):
+        x = torch.as_tensor(np.asarray(x, np.float32))
+    if not x.is_cuda:
+        x = x.to("cuda")
+    x = x.to(torch.float32)
+    module.to_device(x.device.index)
+    return x
+
+
+class RMSNorm(Module):
+    """Root-mean-square norm of each row with a learned ``weight`` [features]
+    (ones).  No counterpart in the reference; f32 features in and out
+    (blocks.rmsNorm has the 16- and 8-bit forms)."""
+
+    def __init__(self, config: Optional[dict] = None, **kw):
+        super().__init__()
+        cfg = dict(config or {})
+        cfg.update(kw)
+        self.features = int(cfg["features"])
+        self.eps = float(cfg.get("eps", 1e-6))
+        self.registerParameter("weight", _torch().ones(self.features))
+
+    def forward(self, input):
+        x = _tensor_on_device(self, input)
+        return _wrap(input, rmsNorm(x, self.p("weight"), eps=self.eps)[0])
+
+    def backward(self, input, grad_out) -> dict:
+        """Gradients of forward(input) for grad_out: {"x", "weight"}."""
+        x = _tensor_on_device(self, input)
+        gx, gw = rmsNormBackward(grad_out, x, self.p("weight"), eps=self.eps)
+        return {"x": gx, "weight": gw}
+
+    def __repr__(self):
+        return f"RMSNorm({self.features})"
+
+
+class GatedFeedForward(Module):
+    """A feed-forward half-block on the features' residual stream, between
+    message-passing layers: x + (act(n gate^T) * (n up^T)) down^T with
+    n = rmsNorm(x, norm).  No counterpart in the reference.
+
+    Features and parameters are f32 (``norm`` [features], ``gate`` and ``up``
+    [hiddenFeatures, features], ``down`` [features, hiddenFeatures]); the
+    products run on the tensor cores with operands in ``type``: "bf16"
+    (default), "f16", or "e4m3" (forward only: the norm's output and the gate
+    and up weights in 8 bits with a scale a row, the rest bf16)."""
+
+    def __init__(self, config: Optional[dict] = None, **kw):
+        super().__init__()
+        torch = _torch()
+        cfg = dict(config or {})
+        cfg.update(kw)
+        self.features = int(cfg["features"])
+        self.hiddenFeatures = int(cfg["hiddenFeatures"])
+        self.act = cfg.get("act", "silu")
+        self.eps = float(cfg.get("eps", 1e-6))
+        self.type = cfg.get("type", "bf16")
+        if self.type not in ("bf16", "f16", "e4m3"):
+            raise ValueError(f"type must be bf16, f16 or e4m3, got {self.type!r}")
+        self.registerParameter("norm", torch.ones(self.features))
+        stdv = np.sqrt(2.0 / (self.features + self.hiddenFeatures))
+        for name in ("gate", "up"):
+            self.registerParameter(name, _param((self.hiddenFeatures, self.features), stdv))
+        self.registerParameter("down", _param((self.features, self.hiddenFeatures), stdv))
+
+    def _half(self):
+        torch = _torch()
+        return torch.float16 if self.type == "f16" else torch.bfloat16
+
+    def _eight(self, name):
+        """A weight in e4m3 with one scale a row."""
+        torch = _torch()
+        w = self.p(name)
+        amax = w.abs().amax(dim=1)
+        scale = torch.where(amax > 0, amax / 448.0, torch.ones_like(amax))
+        return (w / scale[:, None]).to(torch.float8_e4m3fn), scale
+
+    def forward(self, input):
+        torch = _torch()
+        x = _tensor_on_device(self, input)
+        half = self._half()
+        if self.type == "e4m3":
+            n, _, s = rmsNorm(x, self.p("norm"), eps=self.eps, outType=torch.float8_e4m3fn)
+            (g, gs), (u, us) = self._eight("gate"), self._eight("up")
+            h = gatedLinear(n, g, u, act=self.act, xScale=s, gateScale=gs, upScale=us)
+        else:
+            n, _, _ = rmsNorm(x, self.p("norm"), eps=self.eps, outType=half)
+            h = gatedLinear(n, self.p("gate").to(half), self.p("up").to(half), act=self.act)
+        out = linearFused(h, self.p("down").to(half), residual=x, outType=torch.float32)
+        return _wrap(input, out)
+
+    def backward(self, input, grad_out) -> dict:
+        """Gradients of forward(input) for grad_out [rows, features] (f32):
+        {"x", "norm", "gate", "up", "down"}, f32.  The 16-bit activations are
+        computed once more from the input; nothing of the forward is kept."""
+        if self.type == "e4m3":
+            raise NotImplementedError("backward with e4m3 operands: train in bf16 or f16")
+        x = _tensor_on_device(self, input)
+        half = self._half()
+        gate, up, down = (self.p(k).to(half) for k in ("gate", "up", "down"))
+        n, _, _ = rmsNorm(x, self.p("norm"), eps=self.eps, outType=half)
+        h = gatedLinear(n, gate, up, act=self.act)
+        gh, gdown, _ = linearFusedBackward(grad_out.to(half), h, down)
+        gn, ggate, gup, _, _ = gatedLinearBackward(gh, n, gate, up, act=self.act)
+        gx, gnorm = rmsNormBackward(gn, x, self.p("norm"), eps=self.eps, gradTotal=grad_out)
+        return {"x": gx, "norm": gnorm, "gate": ggate.float(), "up": gup.float(),
+                "down": gdown.float()}
+
+    def __repr__(self):
+        return (f"GatedFeedForward({self.features} -> {self.hiddenFeatures} -> {self.features}, "
+                f"{self.act}, {self.type})")
 
 
 register_fusable(Linear)
