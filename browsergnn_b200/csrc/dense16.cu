@@ -80,7 +80,7 @@ struct Maps {
 
 struct GemmArgs {
   uint32_t m, n;          // output size (gated: n columns of h, 2n of the product)
-  uint32_t bn;            // columns of a tile in tensor memory: 32, 64, 128, 256
+  uint32_t bn;            // columns of a tile in tensor memory: 32, 64, 128, 256, 512
   uint32_t stages, stage_bytes;
   uint32_t nkb[2];        // k blocks of each segment (0: no second segment)
   uint32_t batches;       // dw: products that share B (dg^T x, du^T x)
@@ -344,6 +344,20 @@ __device__ __forceinline__ void unit16(const uint4 q, int dt, float (&o)[8]) {
     }
   }
 }
+// `rows` rows of `cols` elements from a slot to rows `pitch` bytes apart, element
+// by element, a row's side by side
+template <class T>
+__device__ __forceinline__ void give_elements(void* slot, char* out, uint64_t pitch, uint32_t lane,
+                                              uint32_t cols, uint32_t rows) {
+  constexpr uint32_t ES = sizeof(T), WIDTH = 64 / ES, STEP = 32 / WIDTH;
+  const uint32_t e = lane % WIDTH;
+  if (e >= cols) return;
+  out += (lane / WIDTH) * pitch + e * ES;
+#pragma unroll 8
+  for (uint32_t r = lane / WIDTH; r < rows; r += STEP, out += STEP * pitch)
+    *reinterpret_cast<T*>(out) = reinterpret_cast<const T*>(
+        slot_unit(slot, (int)r, (int)(e * ES / 16)))[e % (16 / ES)];
+}
 __device__ __forceinline__ void fence_async() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
@@ -412,7 +426,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cta_rank() : 0u;  // of the pair; rank 0 issues the products
   const uint32_t S = g.stages;
-  const uint32_t tmem_cols = 2 * g.bn;
+  const uint32_t bufs = g.bn > 256 ? 1u : 2u;  // accumulators that tensor memory holds
+  const uint32_t tmem_cols = bufs * g.bn;
 
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < S; s++) {
@@ -463,12 +478,14 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (Tiles<EPI, CG> ts(g, wn); ts.more(); ts.next()) {
         const Tile ti = ts.at();
         const int am = (int)(ti.m0 + rank * BM);
-        const int bn0 = (int)(TWO ? ti.n0 : ti.n0 + rank * bl);
+        // a 512-column tile is two products of 256: this CTA's half of each
+        const uint32_t half_b = g.bn > 256 ? 128u : bl;
+        const int bn0 = (int)(TWO && g.bn <= 256 ? ti.n0 : ti.n0 + rank * half_b);
         const uint32_t e = kb_last(ti);
         uint32_t kb = kb_first(ti);
         // dw: the batch's A; else the segment's A and B
         const CUtensorMap* ma = &maps.a[EPI == EPI_PARTIAL ? ti.batch : 0];
-        const CUtensorMap* mb = &maps.b[TWO && CG == 2 ? rank : 0];  // a weight a CTA
+        const CUtensorMap* mb = &maps.b[TWO && CG == 2 && g.bn <= 256 ? rank : 0];  // a weight a CTA
         int k0 = (int)kb * kw;
         for (; kb < e; kb++, k0 += kw) {
           if (EPI != EPI_PARTIAL && !TWO && kb == nkb0) {  // the second segment
@@ -488,7 +505,12 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           if (b_mn) {
             for (uint32_t i = 0; i < bl; i += 64)
-              tma_load_2d<CG>(st + A_BYTES + i * 128, mb, bn0 + (int)i, k0, bar);
+              tma_load_2d<CG>(st + A_BYTES + i * 128, mb,
+                              bn0 + (int)(i < half_b ? i : i + 128), k0, bar);
+          } else if (g.bn > 256) {
+            tma_load_2d<CG>(st + A_BYTES, mb, k0, bn0, bar);
+            tma_load_2d<CG>(st + A_BYTES + 128 * 128, TWO ? &maps.b[1] : mb, k0,
+                            TWO ? bn0 : bn0 + 256, bar);
           } else {
             tma_load_2d<CG>(st + A_BYTES, mb, k0, bn0, bar);
             if (TWO && CG == 1)
@@ -513,7 +535,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint64_t desc_a = smem_desc(base, g.a_mn), desc_b = smem_desc(base + A_BYTES, g.b_mn);
       const uint32_t step_a = (g.a_mn ? 2048u : 32u) >> 4, step_b = (g.b_mn ? 2048u : 32u) >> 4;
       const uint32_t stage16 = g.stage_bytes >> 4, idesc = g.idesc, bn = g.bn;
-      auto issue = [&](auto fp8) -> bool {
+      auto issue = [&](auto fp8, auto wide) -> bool {
         for (Tiles<EPI, CG> ts(g, wn); ts.more(); ts.next()) {
           const Tile ti = ts.at();
           const uint32_t last = kb_last(ti);
@@ -532,19 +554,29 @@ __global__ void __launch_bounds__(THREADS, 1)
               for (uint32_t kk = 0; kk < 4; kk++) {
                 if (decltype(fp8)::value) mma_f8<CG>(d, da + kk * step_a, db + kk * step_b, idesc, acc);
                 else mma_f16<CG>(d, da + kk * step_a, db + kk * step_b, idesc, acc);
+                if (decltype(wide)::value) {  // the second 256 columns; A stays where it is
+                  const uint64_t d2 = db + (128 * 128 >> 4) + kk * step_b;
+                  if (decltype(fp8)::value) mma_f8<CG>(d + 256, da + kk * step_a, d2, idesc, acc);
+                  else mma_f16<CG>(d + 256, da + kk * step_a, d2, idesc, acc);
+                }
                 acc = 1u;
               }
               mma_commit<CG>(b_empty + 8 * s);
               if (++s == S) s = 0, ph ^= 1u;
             }
             mma_commit<CG>(b_accf + 8 * buf);
-            if (++buf == 2) buf = 0, aph ^= 1u;
+            if (++buf == bufs) buf = 0, aph ^= 1u;
           } while (kb < last);
         }
         return true;
       };
-      if (g.fp8) issue(std::true_type{});
-      else issue(std::false_type{});
+      if (CG == 2 && bufs == 1) {
+        if (g.fp8) issue(std::true_type{}, std::true_type{});
+        else issue(std::false_type{}, std::true_type{});
+      } else {
+        if (g.fp8) issue(std::true_type{}, std::false_type{});
+        else issue(std::false_type{}, std::false_type{});
+      }
       // every product issued is done before tensor memory is freed
       mma_commit_here<CG>(b_last);
       mbar_drain(b_last, 0);
@@ -566,7 +598,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_at<CG>(b_acce + 8 * buf);
-      if (++buf == 2) buf = 0, aph ^= 1u;
+      if (++buf == bufs) buf = 0, aph ^= 1u;
     };
     bool gave_up = false;
     for (Tiles<EPI, CG> ts(g, wn); ts.more() && !gave_up; ts.next()) {
@@ -624,37 +656,24 @@ __global__ void __launch_bounds__(THREADS, 1)
       // units, its elements side by side.  (TMA stores of a slot took turns with
       // the ring's loads: gated backward 669 us against 645.)
       auto give_slot = [&](void* out, uint64_t ld, int type, uint32_t col) {
-        char* slot = reinterpret_cast<char*>(slots) + SLOT_BYTES;
         __syncwarp();
-        const uint32_t per = type == BGNN_F32 ? 4u : 8u;  // elements of a unit
-        if (vec_out && col + 4 * per <= g.n) {
-          const uint32_t c = col + (lane & 3) * per;
+        const uint32_t es = type == BGNN_F32 ? 4u : 2u, width = 64u / es;
+        char* at = static_cast<char*>(out) + ((uint64_t)row0 * ld + col) * es;
+        const uint64_t pitch = ld * es;
+        if (vec_out && col + width <= g.n) {
+          const uint4* q = slot_unit(slots + SLOT_BYTES, lane >> 2, lane & 3);
+          at += (lane >> 2) * pitch + (lane & 3) * 16;
+          uint4 v[4];
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const int r = i * 8 + (lane >> 2);
-            const uint4 q = *slot_unit(slot, r, lane & 3);
-            if (row0 + r < g.m)
-              *reinterpret_cast<uint4*>(static_cast<char*>(out) +
-                                        ((uint64_t)(row0 + r) * ld + c) * (16u / per)) = q;
-          }
+          for (int i = 0; i < 4; i++) v[i] = q[i * 32];  // 8 rows on: the same swizzle
+#pragma unroll
+          for (int i = 0; i < 4; i++, at += 8 * pitch)
+            if (row0 + (lane >> 2) + i * 8 < g.m) *reinterpret_cast<uint4*>(at) = v[i];
         } else {
-          const uint32_t e = type == BGNN_F32 ? lane & 15 : lane;  // this lane's column
-          const int rows = type == BGNN_F32 ? 2 : 1;               // rows at once
-          if (col + e < g.n) {
-#pragma unroll 8
-            for (int r = type == BGNN_F32 ? lane >> 4 : 0; r < 32; r += rows) {
-              const char* unit = reinterpret_cast<const char*>(slot_unit(slot, r, e / per));
-              const uint64_t at = (uint64_t)(row0 + r) * ld + col + e;
-              if (row0 + r < g.m) {
-                if (type == BGNN_F32)
-                  static_cast<uint32_t*>(out)[at] =
-                      reinterpret_cast<const uint32_t*>(unit)[e % 4];
-                else
-                  static_cast<uint16_t*>(out)[at] =
-                      reinterpret_cast<const uint16_t*>(unit)[e % 8];
-              }
-            }
-          }
+          const uint32_t cols = g.n - col < width ? g.n - col : width;
+          const uint32_t rows = g.m > row0 ? (g.m - row0 < 32 ? g.m - row0 : 32u) : 0u;
+          if (es == 4) give_elements<uint32_t>(slots + SLOT_BYTES, at, pitch, lane, cols, rows);
+          else give_elements<uint16_t>(slots + SLOT_BYTES, at, pitch, lane, cols, rows);
         }
         __syncwarp();
       };
@@ -662,6 +681,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (type == BGNN_F32) {
 #pragma unroll
           for (int h = 0; h < 2; h++) {
+            if (col0 + 16 * h >= g.n) break;
 #pragma unroll
             for (int u = 0; u < 4; u++)
               *slot_unit(slots + SLOT_BYTES, lane, u) = make_uint4(
@@ -1022,19 +1042,33 @@ struct Shape {
   uint32_t bn;
   int cg;
 };
-// The widest that still gives every SM (pair) a tile, since a wide tile reads
-// A fewer times and a pair reads B once for both; a narrow output takes the
-// narrowest that covers it.
-Shape pick_shape(const bgnn_ctx* ctx, uint64_t m, uint64_t n, uint64_t z, bool two,
-                 uint32_t least) {
-  const uint64_t sms = (uint64_t)ctx->num_sms;
+// 256 columns for a pair while every pair has a tile, since a wide tile reads A
+// fewer times and a pair reads B once for both; below that the widest of one
+// CTA that gives every SM one; a narrow output takes the narrowest that covers
+// it.  512 columns (where may_512) for a long contraction: a k block loads 48 KB a CTA
+// for the products that two 32 KB ones take in 256 columns, and loads bound it (about
+// 48 bytes a clock and SM), but the accumulator fills tensor memory, so that
+// the epilogue does not overlap the next tile.  A 512-column tile takes about
+// WIDE / 100 times a 256-column one.
+constexpr uint64_t WIDE = 160;
+Shape pick_shape(const bgnn_ctx* ctx, uint64_t m, uint64_t n, uint64_t z, bool two, uint32_t least,
+                 uint32_t nkb, bool may_512) {
+  const uint64_t sms = (uint64_t)ctx->num_sms, pairs = sms / 2;
   Shape s = {256, 2};
-  const uint64_t wn = two ? 128 : 256;
-  if (((m + 2 * BM - 1) / (2 * BM)) * ((n + wn - 1) / wn) * z * 2 >= sms && n > wn / 2) return s;
+  auto tiles = [&](uint64_t rows, uint64_t cols) {
+    return ((m + rows - 1) / rows) * ((n + cols - 1) / cols) * z;
+  };
+  const uint64_t wn = two ? 128 : 256, t256 = tiles(2 * BM, wn), t512 = tiles(2 * BM, 2 * wn);
+  if (t256 >= pairs && n > wn / 2) {
+    if (may_512 && nkb >= 64 &&
+        (t512 + pairs - 1) / pairs * WIDE < (t256 + pairs - 1) / pairs * 100)
+      s.bn = 512;
+    return s;
+  }
   s.cg = 1;
   while (s.bn > least) {
     const uint64_t w = two ? s.bn / 2 : s.bn;
-    if (((m + BM - 1) / BM) * ((n + w - 1) / w) * z >= sms && n > w / 2) break;
+    if (tiles(BM, w) >= sms && n > w / 2) break;
     s.bn /= 2;
   }
   return s;
@@ -1051,7 +1085,7 @@ void set_tile(GemmArgs* g, const Shape& s) {
 uint32_t make_idesc(int type, int a_mn, int b_mn, const Shape& s) {
   const uint32_t f = type == BGNN_BF16 ? 1u : 0u;  // kind::f16: 0 f16, 1 bf16; f8f6f4: 0 e4m3
   return (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
-         ((s.bn >> 3) << 17) | ((uint32_t)(BM * s.cg >> 4) << 24);
+         (((s.bn > 256 ? 256 : s.bn) >> 3) << 17) | ((uint32_t)(BM * s.cg >> 4) << 24);
 }
 
 template <int EPI, int CG>
@@ -1124,17 +1158,19 @@ int run_nt(bgnn_ctx* ctx, GemmArgs& g, Mat x, const Mat (&w)[2], uint32_t k) {
   DevTmp tx, tw[2], tin;
   Maps maps;
   g.a_mn = g.b_mn = 0;
-  const Shape sh = pick_shape(ctx, g.m, g.n, 1, TWO, TWO ? 64 : 32);
-  set_tile(&g, sh);
   g.nkb[0] = blocks_of(k, g.in_type == BGNN_E4M3 ? 128 : 64);
   g.nkb[1] = 0;
+  const Shape sh = pick_shape(ctx, g.m, g.n, 1, TWO, TWO ? 64 : 32, g.nkb[0],
+                              EPI != EPI_LINEAR || g.out_type != BGNN_F32);
+  set_tile(&g, sh);
   if (k) {
     BGNN_TRY(tma_ready(ctx, g.in_type, &x, tx));
     BGNN_TRY(make_map(ctx, &maps.a[0], g.in_type, x, BM));
     for (int i = 0; i < (TWO ? 2 : 1); i++) {
       Mat wi = w[i];
       BGNN_TRY(tma_ready(ctx, g.in_type, &wi, tw[i]));
-      BGNN_TRY(make_map(ctx, &maps.b[i], g.in_type, wi, TWO ? g.bn / 2 : g.bn / sh.cg));
+      BGNN_TRY(make_map(ctx, &maps.b[i], g.in_type, wi,
+                        g.bn > 256 ? 128 : TWO ? g.bn / 2 : g.bn / sh.cg));
     }
   }
   if (g.other) {
@@ -1158,7 +1194,7 @@ int run_dx(bgnn_ctx* ctx, int type, uint32_t m, uint32_t n, uint32_t k, const Ma
   g.in_type = type;
   g.a_mn = 0;
   g.b_mn = 1;
-  const Shape sh = pick_shape(ctx, m, k, 1, false, 64);
+  const Shape sh = pick_shape(ctx, m, k, 1, false, 64, blocks_of(n, 64) * terms, true);
   set_tile(&g, sh);
   for (int i = 0; i < terms; i++) {
     Mat a = dz[i], b = w[i];
@@ -1188,8 +1224,12 @@ int run_dw(bgnn_ctx* ctx, int type, uint32_t m, uint32_t n, uint32_t k, const Ma
   g.batches = (uint32_t)terms;
   Shape sh = {k <= 64 ? 64u : k <= 128 ? 128u : 256u, 1};
   if (sh.bn == 256 && n > BM) sh.cg = 2;
-  set_tile(&g, sh);
   g.nkb[0] = blocks_of(m, 64);
+  if (sh.cg == 2) {
+    const Shape wide = pick_shape(ctx, n, k, terms, false, 64, g.nkb[0], true);
+    if (wide.bn == 512) sh = wide;
+  }
+  set_tile(&g, sh);
   // ranges so that every SM has a tile, each of at least 8 k blocks, and of at
   // most MAX_PER: the tensor cores' own additions cost about 2^-24 a block
   const uint64_t tiles = (uint64_t)blocks_of(n, BM * sh.cg) * blocks_of(k, g.bn) * terms;
