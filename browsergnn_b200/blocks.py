@@ -432,7 +432,7 @@ def logProbs(logits, targets, mask=None, topK: int = 0):
     t = _targets(targets, rows)
     m, ldm = _mask(mask, rows, cols)
     dev = _device(logits=x, targets=t, mask=m)
-    logp, ent, lse = (_empty((rows,), torch.float32, x) for _ in range(3))
+    logp, ent, lse = _empty((3, rows), torch.float32, x).unbind(0)
     ids = top = None
     if topK:
         ids = _empty((rows, int(topK)), torch.int32, x)

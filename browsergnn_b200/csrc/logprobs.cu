@@ -232,7 +232,8 @@ struct TopShared {
   float m[LP_WARPS], s[LP_WARPS], w[LP_WARPS];
   float v[CANDS];
   uint32_t id[CANDS];
-  int n;
+  uint32_t key[LP_WARPS * 32], low;
+  int n, reach;  // candidates; threads that reach the border
 };
 // a whole number that orders as the float does; 0: nothing
 __device__ __forceinline__ uint32_t order_key(float v) {
@@ -241,28 +242,46 @@ __device__ __forceinline__ uint32_t order_key(float v) {
   return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 // A border that at least k of the block's keys reach, and not many more: the
-// k-th largest, or its leading bits.  0 when fewer than k keys are not 0.
-__device__ __forceinline__ uint32_t border(uint32_t key, int k) {
-  uint32_t p = 0;
-  for (int bit = 31; bit >= 0; bit--) {
-    const uint32_t q = p | (1u << bit);
-    const int c = __syncthreads_count(key >= q);
-    if (c >= k) {
-      p = q;
-      if (c <= k + 8) break;
+// k-th largest, or its leading bits.  0 when fewer than k keys are not 0.  One
+// warp searches (a barrier a bit took three times as long); all threads get it.
+__device__ __forceinline__ uint32_t border(TopShared& sm, uint32_t key, int k, int warp, int lane) {
+  sm.key[threadIdx.x] = key;
+  __syncthreads();
+  if (warp == 0) {
+    uint32_t q[LP_WARPS];
+#pragma unroll
+    for (int i = 0; i < LP_WARPS; i++) q[i] = sm.key[i * 32 + lane];
+    uint32_t p = 0;
+    for (int bit = 31; bit >= 0; bit--) {
+      const uint32_t t = p | (1u << bit);
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < LP_WARPS; i++) c += q[i] >= t;
+      c = __reduce_add_sync(0xffffffffu, c);
+      if (c >= k) {
+        p = t;
+        if (c <= k + 8) break;
+      }
     }
+    if (lane == 0) sm.low = p;
   }
-  return p;
+  __syncthreads();
+  return sm.low;
 }
-// appends a candidate a lane; all lanes of the warp call
+// appends a candidate a lane; all lanes of the warp call.  (Their order is not
+// kept: candidates are ranked.)
 __device__ __forceinline__ void add_cands(float* vs, uint32_t* ids, int* count, int most, bool in,
                                           float v, uint32_t id, int lane) {
   const uint32_t b = __ballot_sync(0xffffffffu, in);
   if (b == 0) return;
   int at = 0;
-  if (lane == 0) at = atomicAdd(count, __popc(b));  // their order is not kept: they are ranked
+  if (lane == 0) at = atomicAdd(count, __popc(b));
   at = __shfl_sync(0xffffffffu, at, 0) + __popc(b & ((1u << lane) - 1));
   if (in && at < most) vs[at] = v, ids[at] = id;
+}
+__device__ __forceinline__ void add_cand(TopShared& sm, float v, uint32_t id) {
+  const int at = atomicAdd(&sm.n, 1);
+  if (at < CANDS) sm.v[at] = v, sm.id[at] = id;
 }
 // the block's statistics, in every thread
 __device__ __forceinline__ Stat block_stat(TopShared& sm, Stat t, int warp, int lane) {
@@ -319,7 +338,7 @@ __global__ void __launch_bounds__(LP_WARPS * 32) k_logp(const LogpArgs a) {
   const int64_t hi = end < (int64_t)a.cols ? end : (int64_t)a.cols;
   constexpr int STEP = LP_WARPS * 256;
   const int64_t mine = first + warp * 256 + lane * 8;  // this thread's vectors: mine + i * STEP
-  if (threadIdx.x == 0) sm.n = 0;
+  if (threadIdx.x == 0) sm.n = sm.reach = 0;
   Stat t = {-INFINITY, 0.0f, 0.0f};
   {
     int64_t e = mine;
@@ -364,28 +383,25 @@ __global__ void __launch_bounds__(LP_WARPS * 32) k_logp(const LogpArgs a) {
     }
   };
   if (a.top) {
-    const uint32_t low = border(key, a.top);
-    // the threads that reach the border, one after the other: the warp reads
-    // sixteen of the thread's vectors at a time, four elements a lane
-    uint32_t todo = __ballot_sync(0xffffffffu, key >= low && key != 0);
-    while (todo) {
-      const int src = __ffs((int)todo) - 1;
-      todo &= todo - 1;
-      const int64_t base = first + warp * 256 + src * 8;
-      for (int64_t b = base; b < hi; b += 16 * STEP) {
-        float v[4];
-        const int64_t e = b + (int64_t)(lane >> 3) * STEP + (lane & 7);
+    const uint32_t low = border(sm, key, a.top, warp, lane);
+    // The threads that reach the border, one a half-warp: its lanes read sixteen
+    // of the thread's vectors, and the few elements that reach it are taken.
+    if (key >= low && key != 0) sm.key[atomicAdd(&sm.reach, 1)] = threadIdx.x;
+    __syncthreads();
+    const int reach = sm.reach;
+    for (int f = threadIdx.x >> 4; f < reach; f += 2 * LP_WARPS) {
+      int64_t e = first + (int64_t)sm.key[f] * 8 + (lane & 15) * STEP;
+      for (; e < hi; e += 16 * STEP) {
+        float v[8];
+        load_left<DT>(xr, mr, mask_vec, e, lo, hi, v);
+        float cm = v[0];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int64_t q = e + i * (4 * STEP);
-          const bool in = q >= lo && q < hi && !(mr && mr[q]);
-          v[i] = in ? Elt<DT>::get(xr[q]) : -INFINITY;
-        }
+        for (int j = 1; j < 8; j++) cm = fmaxf(cm, v[j]);
+        if (order_key(cm) < low) continue;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const uint32_t k = order_key(v[i]);
-          add_cands(sm.v, sm.id, &sm.n, CANDS, k >= low && k != 0, v[i],
-                    (uint32_t)(e + i * (4 * STEP)), lane);
+        for (int j = 0; j < 8; j++) {
+          const uint32_t k = order_key(v[j]);
+          if (k >= low && k != 0) add_cand(sm, v[j], (uint32_t)(e + j));
         }
       }
     }
@@ -424,7 +440,7 @@ __global__ void __launch_bounds__(LP_WARPS * 32) k_logp_join(const LogpArgs a) {
   __shared__ TopShared sm;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint64_t row = blockIdx.x;
-  if (threadIdx.x == 0) sm.n = 0;
+  if (threadIdx.x == 0) sm.n = sm.reach = 0;
   Stat t = {-INFINITY, 0.0f, 0.0f};
   for (uint32_t s = threadIdx.x; s < a.splits; s += LP_WARPS * 32) {
     const float4 p = a.part[row * a.splits + s];
@@ -438,12 +454,12 @@ __global__ void __launch_bounds__(LP_WARPS * 32) k_logp_join(const LogpArgs a) {
     float m = -INFINITY;
 #pragma unroll 8
     for (uint32_t i = threadIdx.x; i < n; i += LP_WARPS * 32) m = fmaxf(m, pv[i]);
-    const uint32_t low = border(order_key(m), a.top);
-    for (uint32_t b = warp * 32; b < n; b += LP_WARPS * 32) {
-      const float v = b + lane < n ? pv[b + lane] : -INFINITY;
+    const uint32_t low = border(sm, order_key(m), a.top, warp, lane);
+#pragma unroll 8
+    for (uint32_t i = threadIdx.x; i < n; i += LP_WARPS * 32) {
+      const float v = pv[i];
       const uint32_t k = order_key(v);
-      const bool in = k >= low && k != 0;
-      add_cands(sm.v, sm.id, &sm.n, CANDS, in, v, in ? pi[b + lane] : NO_CHOICE, lane);
+      if (k >= low && k != 0) add_cand(sm, v, pi[i]);
     }
     __syncthreads();
     if (sm.n <= CANDS) {
