@@ -102,6 +102,7 @@ struct GemmArgs {
   int out_type;
   void* out[2];           // gated backward: dg and du; dw: one a batch
   uint64_t ld_out;
+  float* bsum[2];         // backward: column sums of 32 rows each, [rows / 32, n], or NULL
   float* part;            // EPI_PARTIAL: [splits, batches, m, ld_out]; NULL: dw whole, no parts
   int* err;
 };
@@ -365,6 +366,21 @@ __device__ __forceinline__ void fence_async() {
 // whether 16 bytes of a row, from a multiple of as many, are one access
 __device__ __forceinline__ bool vec16_ok(const void* p, int dt, uint64_t ld) {
   return ((uintptr_t)p & 15u) == 0 && ld % (dt == BGNN_F32 ? 4 : 8) == 0;
+}
+
+// Lane j gets the sum over the warp's lanes of v[j]: halves of the columns are
+// handed over at distances 16, 8, .. 1.  v is used up.
+__device__ __forceinline__ float column_sum(float (&v)[32], int lane) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int i = 0; i < o; i++) {
+      const float give = up ? v[i] : v[i + o];
+      v[i] = (up ? v[i + o] : v[i]) + __shfl_xor_sync(0xffffffffu, give, o);
+    }
+  }
+  return v[0];
 }
 
 // the tiles of a CTA (pair), columns fastest
@@ -710,6 +726,13 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int j = 0; j < 32; j++) v[j] += __shfl_sync(0xffffffffu, bv, j);
         }
       };
+      // the bias gradient's share of a chunk, before dz is rounded
+      auto bias_sums = [&](float (&v)[32], uint32_t col0, float* bsum) {
+        if (!bsum) return;
+        const float t = column_sum(v, lane);
+        if (col0 + lane < g.n && row0 < g.m)
+          bsum[(uint64_t)(row0 / 32) * g.n + col0 + lane] = t;
+      };
       auto linear_out = [&](float (&v)[32], uint32_t col0) {
         scaled(v, col0, 0);
         if (g.act != BGNN_ACT_NONE)
@@ -814,6 +837,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               for (int j = 0; j < 8; j++) v[j0 + j] *= o[j];
             });
             give(v, col0, g.out[0], g.ld_out, g.out_type);
+            bias_sums(v, col0, g.bsum[0]);
           } else if constexpr (EPI == EPI_GATED) {
             scaled(v, col0, 0);
             scaled(u, col0, 1);
@@ -851,6 +875,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             });
             give(v, col0, g.out[0], g.ld_out, g.out_type);
             give(u, col0, g.out[1], g.ld_out, g.out_type);
+            bias_sums(v, col0, g.bsum[0]);
+            bias_sums(u, col0, g.bsum[1]);
           }
         }
         release();
@@ -1407,7 +1433,10 @@ extern "C" int bgnn_linear_fused_backward(bgnn_ctx* ctx, int type, const void* g
   }
   const uint32_t ldz = (n + 7) / 8 * 8;
   Mat dz[2] = {{grad, m, n, ld_grad}, {}};
-  DevTmp tz, tg;
+  DevTmp tz, tg, tb;
+  // what the bias gradient sums: dz in f32, 32 rows at a time, or the gradient
+  Mat bsum = dz[0];
+  int bsum_type = type;
   if (m) BGNN_TRY(tma_ready(ctx, type, &dz[0], tg));  // once for every product that reads it
   if (act != BGNN_ACT_NONE && m) {
     BGNN_TRY(bgnn_tmp_alloc(ctx, tz, m * ldz * 2));
@@ -1425,6 +1454,13 @@ extern "C" int bgnn_linear_fused_backward(bgnn_ctx* ctx, int type, const void* g
     g.out_type = type;
     g.out[0] = tz.p;
     g.ld_out = ldz;
+    if (grad_bias) {
+      const uint64_t parts = (m + 31) / 32;
+      BGNN_TRY(bgnn_tmp_alloc(ctx, tb, parts * n * sizeof(float)));
+      g.bsum[0] = tb.as<float>();
+      bsum = {tb.p, parts, n, n};
+      bsum_type = BGNN_F32;
+    }
     const Mat ws[2] = {{w, n, k, ld_w}, {w, n, k, ld_w}};
     BGNN_TRY(run_nt<EPI_LINEAR_BWD>(ctx, g, {x, m, k, ld_x}, ws, k));
     dz[0] = {tz.p, m, n, ldz};
@@ -1435,7 +1471,7 @@ extern "C" int bgnn_linear_fused_backward(bgnn_ctx* ctx, int type, const void* g
     void* const dw[2] = {grad_w, nullptr};
     BGNN_TRY(run_dw(ctx, type, (uint32_t)m, n, k, dz, {x, m, k, ld_x}, 1, dw));
   }
-  if (grad_bias) BGNN_TRY(run_db(ctx, type, dz[0], grad_bias, bias_type));
+  if (grad_bias) BGNN_TRY(run_db(ctx, bsum_type, bsum, grad_bias, bias_type));
   return BGNN_OK;
 }
 
@@ -1462,7 +1498,8 @@ extern "C" int bgnn_gated_linear_backward(bgnn_ctx* ctx, int type, const void* g
     return BGNN_OK;
   }
   const uint32_t ldz = (n + 7) / 8 * 8;
-  DevTmp tz;
+  DevTmp tz, tb[2];
+  const uint64_t parts = (m + 31) / 32;  // of the bias gradients' sums
   BGNN_TRY(bgnn_tmp_alloc(ctx, tz, 2 * m * ldz * 2));
   uint16_t* z0 = tz.as<uint16_t>();
   uint16_t* z1 = z0 + m * ldz;
@@ -1484,6 +1521,11 @@ extern "C" int bgnn_gated_linear_backward(bgnn_ctx* ctx, int type, const void* g
     g.out[0] = z0;
     g.out[1] = z1;
     g.ld_out = ldz;
+    for (int i = 0; i < 2; i++)
+      if (i ? grad_bias_up : grad_bias_gate) {
+        BGNN_TRY(bgnn_tmp_alloc(ctx, tb[i], parts * n * sizeof(float)));
+        g.bsum[i] = tb[i].as<float>();
+      }
     BGNN_TRY(run_nt<EPI_GATED_BWD>(ctx, g, {x, m, k, ld_x}, ws, k));
   }
   const Mat dz[2] = {{z0, m, n, ldz}, {z1, m, n, ldz}};
@@ -1492,7 +1534,9 @@ extern "C" int bgnn_gated_linear_backward(bgnn_ctx* ctx, int type, const void* g
     void* const dw[2] = {grad_w_gate, grad_w_up};
     BGNN_TRY(run_dw(ctx, type, (uint32_t)m, n, k, dz, {x, m, k, ld_x}, 2, dw));
   }
-  if (grad_bias_gate) BGNN_TRY(run_db(ctx, type, dz[0], grad_bias_gate, bias_type));
-  if (grad_bias_up) BGNN_TRY(run_db(ctx, type, dz[1], grad_bias_up, bias_type));
+  if (grad_bias_gate)
+    BGNN_TRY(run_db(ctx, BGNN_F32, {tb[0].p, parts, n, n}, grad_bias_gate, bias_type));
+  if (grad_bias_up)
+    BGNN_TRY(run_db(ctx, BGNN_F32, {tb[1].p, parts, n, n}, grad_bias_up, bias_type));
   return BGNN_OK;
 }

@@ -600,7 +600,7 @@ BGNN_API int bgnn_linear_fused(bgnn_ctx* ctx, int type, const void* x, uint64_t 
 /* Its gradients for an upstream gradient grad [m, n] (type bf16 or f16, as x
  * and w): with z = x w^T + bias computed once more and dz = grad act'(z)
  * rounded to `type`, grad_x = dz w, grad_w = dz^T x (both in `type`),
- * grad_bias = column sums of dz (bias_type).  The residual's gradient is grad.
+ * grad_bias = column sums of the unrounded dz (bias_type).  The residual's gradient is grad.
  * Any of the three may be NULL.  Sums run in a fixed order. */
 BGNN_API int bgnn_linear_fused_backward(bgnn_ctx* ctx, int type, const void* grad,
                                         uint64_t ld_grad, const void* x, uint64_t ld_x,
