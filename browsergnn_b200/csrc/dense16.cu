@@ -616,7 +616,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (lane == 0) mbar_arrive_at<CG>(b_acce + 8 * buf);
       if (++buf == bufs) buf = 0, aph ^= 1u;
     };
-    bool gave_up = false;
+    bool gave_up = false, pending = false;  // pending: a slot was asked for
     for (Tiles<EPI, CG> ts(g, wn); ts.more() && !gave_up; ts.next()) {
       const Tile ti = ts.at();
       const uint32_t k_first = kb_first(ti), k_last = kb_last(ti);
@@ -626,14 +626,20 @@ __global__ void __launch_bounds__(THREADS, 1)
       // Asks for 32 columns (f32: 16) of the residual / upstream gradient into
       // slot 0, with which every lane is done.
       auto ask = [&](uint32_t col) {
-        if (g.other && lane == 0 && col < g.n) {
+        if (!g.other || col >= g.n) return;
+        pending = true;
+        if (lane == 0) {
           fence_async();
           mbar_expect_tx(in_bar, SLOT_BYTES);
           tma_load_2d<1>(s_addr(slots), &maps.in, (int)col, (int)row0, in_bar);
         }
       };
       auto asked = [&]() {
-        if (!mbar_wait(in_bar, in_ph, abort_flag, g.err, 74)) gave_up = true;
+        if (!mbar_wait(in_bar, in_ph, abort_flag, g.err, 74)) {
+          gave_up = true;
+          mbar_drain(in_bar, in_ph);
+        }
+        pending = false;
         in_ph ^= 1u;
       };
       // f(first column, 8 values) for this lane's row of the chunk at col0, eight
@@ -882,6 +888,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         release();
       }
     }
+    if (pending) mbar_drain(in_bar, in_ph);  // gave up: the copy lands before the CTA ends
   }
   pair_sync<CG>();
   if (warp == EPI_WARPS) {
@@ -1114,8 +1121,22 @@ uint32_t make_idesc(int type, int a_mn, int b_mn, const Shape& s) {
          (((s.bn > 256 ? 256 : s.bn) >> 3) << 17) | ((uint32_t)(BM * s.cg >> 4) << 24);
 }
 
+// Registers a thread that an instance was compiled to (the same on every
+// device); setmaxnreg waits for good unless the launch holds what the epilogue
+// and the issuing warps are given.
+template <int EPI, int CG>
+int compiled_regs() {
+  static const int regs = [] {
+    cudaFuncAttributes at;
+    return cudaFuncGetAttributes(&at, k_dense16<EPI, CG>) == cudaSuccess ? at.numRegs : 0;
+  }();
+  return regs;
+}
 template <int EPI, int CG>
 int launch_cg(bgnn_ctx* ctx, const Maps& maps, const GemmArgs& g, uint64_t tiles) {
+  if (compiled_regs<EPI, CG>() * THREADS < (EPI_WARPS * EPI_REGS + 4 * ISSUE_REGS) * 32)
+    return bgnn_set_error(ctx, BGNN_ERR_UNSUPPORTED, "product kernel compiled to %d registers",
+                          compiled_regs<EPI, CG>());
   BGNN_CUDA(ctx, cudaFuncSetAttribute(k_dense16<EPI, CG>,
                                       cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
   const int sms = ctx->grid_sms > 0 && ctx->grid_sms < ctx->num_sms ? ctx->grid_sms : ctx->num_sms;

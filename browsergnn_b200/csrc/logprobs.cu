@@ -604,7 +604,10 @@ __global__ void __launch_bounds__(256) k_logp_bwd_short(const LogpBwdArgs a) {
     };
     if (fabsf(ls) >= LSE_EXACT && fabsf(ls) < INFINITY) {
       Stat t = {-INFINITY, 0.0f, 0.0f};
-      for (uint32_t e = lane; e < a.cols; e += 32) t = stat_merge(t, {at(e), 1.0f, 0.0f});
+      for (uint32_t e = lane; e < a.cols; e += 32) {
+        const float x = at(e);
+        if (x > -INFINITY) t = stat_merge(t, {x, 1.0f, 0.0f});
+      }
       t = warp_stat(t);
       m = t.m;
       ls = logf(t.s);

@@ -531,6 +531,69 @@ def test_log_probs_ties_lowest_values_and_not_finite():
     assert logp.tolist() == [0, 0] and ent.tolist() == [0, 0] and (ids == -1).all()
 
 
+@pytest.mark.parametrize("cols", [40, 700, 3000])
+@pytest.mark.parametrize("at", [500.0, -3e4])
+def test_log_probs_far_from_zero(cols, at):
+    """Rows whose log-sum-exp is large, masks among them: the gradient does not
+    lean on its last bits."""
+    g = gen(cols)
+    x = normal(g, 6, cols) + at
+    m = torch.rand(6, cols, device="cuda", generator=g) < 0.4
+    m[5] = True
+    t = torch.zeros(6, device="cuda", dtype=torch.int64)
+    logp, ent, lse, _, _ = bg.logProbs(x, t, mask=m)
+    lp, p, lse_w, logp_w, ent_w, _, _ = head64(x, m, t, 1)
+    within(logp, logp_w, 2.0 ** -18 * (1 + logp_w.abs().nan_to_num(posinf=0)), "logp")
+    within(ent, ent_w, 2.0 ** -18 * (1 + ent_w), "entropy")
+    gl = torch.ones(6, device="cuda")
+    d = bg.logProbsBackward(x, t, lse, ent, gl, mask=m)
+    hit = torch.zeros_like(p)
+    hit[:, 0] = (left64(x, m)[:, 0] > -math.inf).double()
+    # p from m and S summed again in f32: 2^-18 of it is more than their error
+    within(d, hit - p, 2.0 ** -18 * p + 2.0 ** -23, "logits")
+
+
+def test_gated_with_one_bias():
+    g = gen(77)
+    x, wg, wu = normal(g, 40, 64, t=BF), normal(g, 48, 64, t=BF), normal(g, 48, 64, t=BF)
+    b, zero = normal(g, 48, t=BF), torch.zeros(48, device="cuda", dtype=BF)
+    go = normal(g, 40, 48, t=BF)
+    for rows in (1, 40):
+        xs, gs = x[:rows], go[:rows]
+        assert torch.equal(bg.gatedLinear(xs, wg, wu, biasGate=b),
+                           bg.gatedLinear(xs, wg, wu, biasGate=b, biasUp=zero))
+        assert torch.equal(bg.gatedLinear(xs, wg, wu, biasUp=b),
+                           bg.gatedLinear(xs, wg, wu, biasGate=zero, biasUp=b))
+        one = bg.gatedLinearBackward(gs, xs, wg, wu, biasUp=b)
+        two = bg.gatedLinearBackward(gs, xs, wg, wu, biasGate=zero, biasUp=b)
+        assert one[3] is None
+        for i in (0, 1, 2, 4):
+            assert torch.equal(one[i], two[i])
+
+
+def test_long_contractions_take_the_wide_tiles():
+    """512-column tiles (operands of both majors, ragged edges) against the
+    64-bit product."""
+    g = gen(5)
+    # 18 x 16 tiles of 256 columns on 74 pairs: four rounds, two of 512 columns
+    m, k, n = 4500, 4088, 4088
+    x, w = normal(g, m, k, t=BF), normal(g, n, k, t=BF, std=k ** -0.5)
+    go = normal(g, m, n, t=BF)
+    out = bg.linearFused(x, w)
+    want = x.double() @ w.double().t()
+    S = x.double().abs() @ w.double().abs().t()
+    within(out, want, acc(k) * S + (U[BF] + U[F32]) * want.abs(), "out")
+    gx, gw, _ = bg.linearFusedBackward(go, x, w)
+    G = go.double()
+    want = G @ w.double()
+    within(gx, want, acc(n) * (G.abs() @ w.double().abs()) + (U[BF] + U[F32]) * want.abs(), "x")
+    want = G.t() @ x.double()
+    within(gw, want, acc(m) * (G.abs().t() @ x.double().abs()) + (U[BF] + U[F32]) * want.abs(), "w")
+    test_gated_linear(m, k, 2040, BF, "silu", BF, "plain")
+    test_gated_linear(m, 8200, 2036, F8, "gelu", None, "plain")
+    test_gated_linear_backward(m, k, 2040, F16, "gelu", F16, "plain")
+
+
 def test_log_probs_target_out_of_range():
     ctx = bg.get_context()
     ctx.synchronize()
