@@ -41,6 +41,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <atomic>
 #include <cstring>
 #include <mutex>
 
@@ -1137,8 +1138,13 @@ int launch_cg(bgnn_ctx* ctx, const Maps& maps, const GemmArgs& g, uint64_t tiles
   if (compiled_regs<EPI, CG>() * THREADS < (EPI_WARPS * EPI_REGS + 4 * ISSUE_REGS) * 32)
     return bgnn_set_error(ctx, BGNN_ERR_UNSUPPORTED, "product kernel compiled to %d registers",
                           compiled_regs<EPI, CG>());
-  BGNN_CUDA(ctx, cudaFuncSetAttribute(k_dense16<EPI, CG>,
-                                      cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
+  static std::atomic<uint64_t> ready{0};  // devices (below 64) whose limit is set
+  const uint64_t bit = ctx->device < 64 ? 1ull << ctx->device : 0;
+  if (!(ready.load(std::memory_order_relaxed) & bit)) {
+    BGNN_CUDA(ctx, cudaFuncSetAttribute(k_dense16<EPI, CG>,
+                                        cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
   const int sms = ctx->grid_sms > 0 && ctx->grid_sms < ctx->num_sms ? ctx->grid_sms : ctx->num_sms;
   const uint64_t most = sms / CG > 0 ? sms / CG : 1;
   cudaLaunchConfig_t cfg = {};
@@ -1325,6 +1331,9 @@ int run_db(bgnn_ctx* ctx, int type, const Mat& dz, void* db, int db_type) {
     BGNN_CUDA(ctx, cudaMemsetAsync(db, 0, dz.cols * dtype_size(db_type), ctx->stream));
     return BGNN_OK;
   }
+  if (type == BGNN_F32 && dz.ld == dz.cols && dz.rows <= 2048)  // few sums: one kernel
+    return bgnn_run_sum_parts(ctx, static_cast<const float*>(dz.p), (uint32_t)dz.rows, dz.cols, db,
+                              db_type);
   const uint32_t cb = blocks_of(dz.cols, 32);
   uint64_t parts = ((uint64_t)ctx->num_sms * 8 + cb - 1) / cb;
   const uint64_t most = (dz.rows + 63) / 64;
@@ -1454,13 +1463,14 @@ extern "C" int bgnn_linear_fused_backward(bgnn_ctx* ctx, int type, const void* g
   }
   const uint32_t ldz = (n + 7) / 8 * 8;
   Mat dz[2] = {{grad, m, n, ld_grad}, {}};
-  DevTmp tz, tg, tb;
+  DevTmp tz, tg;
   // what the bias gradient sums: dz in f32, 32 rows at a time, or the gradient
   Mat bsum = dz[0];
   int bsum_type = type;
   if (m) BGNN_TRY(tma_ready(ctx, type, &dz[0], tg));  // once for every product that reads it
   if (act != BGNN_ACT_NONE && m) {
-    BGNN_TRY(bgnn_tmp_alloc(ctx, tz, m * ldz * 2));
+    const uint64_t parts = grad_bias ? (m + 31) / 32 : 0;
+    BGNN_TRY(bgnn_tmp_alloc(ctx, tz, m * ldz * 2 + parts * n * sizeof(float)));
     GemmArgs g = {};
     g.m = (uint32_t)m;
     g.n = n;
@@ -1476,10 +1486,8 @@ extern "C" int bgnn_linear_fused_backward(bgnn_ctx* ctx, int type, const void* g
     g.out[0] = tz.p;
     g.ld_out = ldz;
     if (grad_bias) {
-      const uint64_t parts = (m + 31) / 32;
-      BGNN_TRY(bgnn_tmp_alloc(ctx, tb, parts * n * sizeof(float)));
-      g.bsum[0] = tb.as<float>();
-      bsum = {tb.p, parts, n, n};
+      g.bsum[0] = reinterpret_cast<float*>(tz.as<uint16_t>() + m * ldz);
+      bsum = {g.bsum[0], parts, n, n};
       bsum_type = BGNN_F32;
     }
     const Mat ws[2] = {{w, n, k, ld_w}, {w, n, k, ld_w}};
@@ -1519,11 +1527,15 @@ extern "C" int bgnn_gated_linear_backward(bgnn_ctx* ctx, int type, const void* g
     return BGNN_OK;
   }
   const uint32_t ldz = (n + 7) / 8 * 8;
-  DevTmp tz, tb[2];
-  const uint64_t parts = (m + 31) / 32;  // of the bias gradients' sums
-  BGNN_TRY(bgnn_tmp_alloc(ctx, tz, 2 * m * ldz * 2));
+  DevTmp tz;  // dg, du, then the bias gradients' sums of 32 rows
+  const uint64_t parts = (m + 31) / 32;
+  BGNN_TRY(bgnn_tmp_alloc(ctx, tz, 2 * m * ldz * 2 +
+                                       (grad_bias_gate || grad_bias_up ? 2 * parts * n * 4 : 0)));
   uint16_t* z0 = tz.as<uint16_t>();
   uint16_t* z1 = z0 + m * ldz;
+  float* sums[2];
+  sums[0] = reinterpret_cast<float*>(z1 + m * ldz);
+  sums[1] = sums[0] + parts * n;
   const Mat ws[2] = {{w_gate, n, k, ld_gate}, {w_up, n, k, ld_up}};
   if (m) {
     GemmArgs g = {};
@@ -1542,11 +1554,8 @@ extern "C" int bgnn_gated_linear_backward(bgnn_ctx* ctx, int type, const void* g
     g.out[0] = z0;
     g.out[1] = z1;
     g.ld_out = ldz;
-    for (int i = 0; i < 2; i++)
-      if (i ? grad_bias_up : grad_bias_gate) {
-        BGNN_TRY(bgnn_tmp_alloc(ctx, tb[i], parts * n * sizeof(float)));
-        g.bsum[i] = tb[i].as<float>();
-      }
+    g.bsum[0] = grad_bias_gate ? sums[0] : nullptr;
+    g.bsum[1] = grad_bias_up ? sums[1] : nullptr;
     BGNN_TRY(run_nt<EPI_GATED_BWD>(ctx, g, {x, m, k, ld_x}, ws, k));
   }
   const Mat dz[2] = {{z0, m, n, ldz}, {z1, m, n, ldz}};
@@ -1556,8 +1565,8 @@ extern "C" int bgnn_gated_linear_backward(bgnn_ctx* ctx, int type, const void* g
     BGNN_TRY(run_dw(ctx, type, (uint32_t)m, n, k, dz, {x, m, k, ld_x}, 2, dw));
   }
   if (grad_bias_gate)
-    BGNN_TRY(run_db(ctx, BGNN_F32, {tb[0].p, parts, n, n}, grad_bias_gate, bias_type));
+    BGNN_TRY(run_db(ctx, BGNN_F32, {sums[0], parts, n, n}, grad_bias_gate, bias_type));
   if (grad_bias_up)
-    BGNN_TRY(run_db(ctx, BGNN_F32, {tb[1].p, parts, n, n}, grad_bias_up, bias_type));
+    BGNN_TRY(run_db(ctx, BGNN_F32, {sums[1], parts, n, n}, grad_bias_up, bias_type));
   return BGNN_OK;
 }
