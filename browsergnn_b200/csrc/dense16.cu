@@ -1182,7 +1182,7 @@ template <int EPI>
 int run_nt(bgnn_ctx* ctx, GemmArgs& g, Mat x, const Mat (&w)[2], uint32_t k) {
   constexpr bool TWO = EPI == EPI_GATED || EPI == EPI_GATED_BWD;
   if constexpr (EPI == EPI_LINEAR || EPI == EPI_GATED)
-    if (g.m <= FEW_ROWS) {
+    if (few_rows(g.m, k, g.n, TWO)) {
       RowsArgs r = {};
       r.x = x.p;
       r.ld_x = x.ld;

@@ -7,7 +7,8 @@
 // lanes stream the weight's row (rows) in 16-byte pieces, several in flight,
 // multiply with the rows of x (which stay in L1), and add up in f32: one chain
 // a lane, then a tree of shuffles.  Rows that do not start on 16 bytes are read
-// an element a lane.
+// an element a lane.  Small products of more rows run here too, eight rows a
+// block: no tensor maps, no copies of rows that TMA cannot take.
 #include "lowp.cuh"
 
 #include "dense_rows.cuh"
@@ -51,10 +52,11 @@ __global__ void __launch_bounds__(WARPS * 32) k_dense_rows(const RowsArgs a) {
   w[0] = static_cast<const char*>(a.w[0]) + (uint64_t)col * a.ld_w[0] * ES;
   w[1] = TWO ? static_cast<const char*>(a.w[1]) + (uint64_t)col * a.ld_w[1] * ES : nullptr;
   const char* x[M];
+  const uint32_t row0 = blockIdx.y * M, rows = a.m - row0 < M ? a.m - row0 : M;
 #pragma unroll
   for (int i = 0; i < M; i++)  // a row that is not there repeats the last
     x[i] = static_cast<const char*>(a.x) +
-           (uint64_t)(i < (int)a.m ? i : (int)a.m - 1) * a.ld_x * ES;
+           (uint64_t)(row0 + ((uint32_t)i < rows ? i : rows - 1)) * a.ld_x * ES;
   float s[TWO ? 2 : 1][M];
 #pragma unroll
   for (int t = 0; t < (TWO ? 2 : 1); t++)
@@ -119,10 +121,11 @@ __global__ void __launch_bounds__(WARPS * 32) k_dense_rows(const RowsArgs a) {
       z0 = s[0][i];
       if (TWO) z1 = s[TWO][i];
     }
-  if (lane >= (int)a.m) return;
+  if ((uint32_t)lane >= rows) return;
+  const uint64_t row = row0 + lane;
   if (DT == BGNN_E4M3) {
-    z0 *= a.x_scale[lane] * a.w_scale[0][col];
-    if (TWO) z1 *= a.x_scale[lane] * a.w_scale[1][col];
+    z0 *= a.x_scale[row] * a.w_scale[0][col];
+    if (TWO) z1 *= a.x_scale[row] * a.w_scale[1][col];
   }
   if (a.bias[0]) z0 += load_any(a.bias[0], a.bias_type, col);
   if (TWO && a.bias[1]) z1 += load_any(a.bias[1], a.bias_type, col);
@@ -131,13 +134,13 @@ __global__ void __launch_bounds__(WARPS * 32) k_dense_rows(const RowsArgs a) {
     o = act_two<decltype(act)::value>(make_float2(z0, 0.0f), a.act_p).x;
   });
   if (TWO) o *= z1;
-  else if (a.other) o += load_any(a.other, a.other_type, (uint64_t)lane * a.ld_other + col);
-  store_any(a.out, a.out_type, (uint64_t)lane * a.ld_out + col, o);
+  else if (a.other) o += load_any(a.other, a.other_type, row * a.ld_other + col);
+  store_any(a.out, a.out_type, row * a.ld_out + col, o);
 }
 
 template <int DT, int M, bool TWO>
 int launch_vec(bgnn_ctx* ctx, const RowsArgs& a, bool vec) {
-  const unsigned grid = (a.n + WARPS - 1) / WARPS;
+  const dim3 grid((a.n + WARPS - 1) / WARPS, (a.m + M - 1) / M);
   constexpr int VEC = DT == BGNN_E4M3 ? 16 : 8;
   if (vec) k_dense_rows<DT, M, TWO, VEC><<<grid, WARPS * 32, 0, ctx->stream>>>(a);
   else k_dense_rows<DT, M, TWO, 1><<<grid, WARPS * 32, 0, ctx->stream>>>(a);

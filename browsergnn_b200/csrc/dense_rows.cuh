@@ -3,9 +3,16 @@
 
 #include "act.cuh"
 
-// Rows up to which they run there: the warps stream the weights in less than
-// the tensor-core kernel's pipeline takes to fill.
+// Up to eight rows always run there: the warps stream the weights in less time
+// than the tensor-core kernel's pipeline takes to fill (1 x 1,024 -> 2 x 4,096:
+// 3.6 us against 10.8; 8 x 4,096 -> 4,096: 20 against 27).  So do small products
+// of more rows: at 64 x 512 -> 512 it is 5.8 us against 6.8, at 16 x 2,048 ->
+// 512 6.3 against 13; twice the outputs (512 x 128 -> 128) take 6.8 against 5.2.
 constexpr uint32_t FEW_ROWS = 8;
+constexpr uint64_t SMALL_OUT = 1ull << 15, SMALL_MACS = 1ull << 24;
+inline bool few_rows(uint64_t m, uint64_t k, uint64_t n, bool two) {
+  return m <= FEW_ROWS || (m * n <= SMALL_OUT && m * n * k * (two ? 2 : 1) <= SMALL_MACS);
+}
 
 struct RowsArgs {
   const void* x;
@@ -27,5 +34,5 @@ struct RowsArgs {
   void* out;
   uint64_t ld_out;
 };
-// 1 <= m <= FEW_ROWS, n >= 1
+// where few_rows says so; m, n >= 1
 int bgnn_run_dense_rows(bgnn_ctx* ctx, int type, const RowsArgs& a);

@@ -226,6 +226,10 @@ PRODUCTS = [  # m, k, n, type, act, bias, residual, out
     (3, 75, 130, F8, None, None, None, F32), (4, 0, 9, F16, "sigmoid", F16, None, F16),
     (5, 2050, 33, BF, "relu", F32, BF, F32), (1, 4096, 4100, BF, "silu", None, None, BF),
     (8, 300, 64, F16, "tanh", None, F16, F16), (9, 300, 64, F16, "tanh", None, F16, F16),
+    # small enough for the rows' kernel, and just not
+    (1001, 40, 32, BF, "silu", BF, F32, F32), (1025, 40, 32, BF, "silu", BF, F32, F32),
+    (21, 9000, 88, F16, None, None, None, F32), (21, 9100, 88, F16, None, None, None, F32),
+    (700, 130, 120, F8, "gelu", BF, BF, BF),
 ]
 
 
