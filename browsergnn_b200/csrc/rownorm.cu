@@ -18,8 +18,9 @@
 // vectors of eight columns, so that its sums are shuffles; longer rows to
 // several warps and one barrier a sum.  Rows that do not start on 16 bytes (an
 // odd width) are read as aligned 16-byte words shifted into place, and leave
-// through shared memory the same way: element by element they ran at 0.56 TB/s
-// (20,000 x 1,433 f16 backward) and 1.6 TB/s (forward).  Rows longer than the
+// through shared memory the same way: 2.4 TB/s at 20,000 x 1,433 f16 backward
+// (4.3 aligned, at 1,432 columns); element by element 0.56.  2.45M x 256 f32 with
+// an f32 residual: 6.0 TB/s, 92 % of what a copy reaches.  Rows longer than the
 // registers of a block hold (RowShape) take the k_*_long kernels, which read
 // the row again from L2.
 #include "lowp.cuh"
