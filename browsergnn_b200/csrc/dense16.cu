@@ -23,9 +23,10 @@
 //   warps 0-15 epilogue: warp w takes the accumulator lanes (rows) of its
 //             quadrant w % 4 and every fourth 32-column chunk; a chunk of the
 //             residual comes by TMA into one shared-memory slot, the result
-//             goes out through the other, turned round to run along rows.  Sixteen warps, four a scheduler: with eight
-//             the activations of a short contraction ran at a third of the
-//             issue rate and bound the kernel.
+//             goes out through the other, turned round to run along rows.
+//             Sixteen warps, four a scheduler: with eight the activations of a
+//             short contraction ran at a third of the issue rate and bound the
+//             kernel.
 // An operand whose contraction runs down its rows (w in dx, both in dw) is
 // read as it lies ("MN-major": boxes of 64 columns x 64 rows), never
 // transposed in memory.  The gated kernels load BN/2 rows of each weight side
@@ -70,14 +71,21 @@ static_assert(SMEM_BYTES <= 227 * 1024, "shared memory of one SM");
 constexpr uint32_t SPIN_LIMIT = 1u << 24;     // polls before a wait gives up,
 constexpr long long SPIN_CLOCKS = 4000000000ll;  // or clocks (about two seconds)
 
-enum Epi : int { EPI_LINEAR, EPI_LINEAR_F32, EPI_GATED, EPI_LINEAR_BWD, EPI_GATED_BWD, EPI_PARTIAL };
+enum Epi : int {
+  EPI_LINEAR,
+  EPI_LINEAR_F32,
+  EPI_GATED,
+  EPI_LINEAR_BWD,
+  EPI_GATED_BWD,
+  EPI_PARTIAL
+};
 // k blocks whose products one accumulator takes before they are added in f32
 // registers, where the result stays f32 (EPI_LINEAR_F32)
 constexpr uint32_t PIECE = 8;
 constexpr uint32_t MAX_PER = 512;  // k blocks of a dw range
 
-// One contraction segment: A [m, k] and B [n, k] tiles of one or two tensors.
-// Where `b1` is used (gated), B's tile is rows of b0 above rows of b1.
+// a, b: the operands of each contraction segment (dx), of each batch (dw: a), or
+// the two weights of a gated product (b).
 // in: the residual or upstream gradient in boxes of a slot.
 struct Maps {
   CUtensorMap a[2], b[2], in;
@@ -485,124 +493,124 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   if (warp >= EPI_WARPS) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(ISSUE_REGS));
-  if (warp == EPI_WARPS) {
-    // ---- TMA producer ----
-    if (lane == 0) {
-      uint32_t s = 0, ph = 0, st = base;
-      uint64_t filled = 0;
-      const uint32_t tx = CG * (A_BYTES + bl * 128);
-      const int kw = g.fp8 ? 128 : 64;  // elements of a k block
-      // both CTAs' loads count on the issuing CTA's barriers
-      const uint32_t b_land = CG == 2 ? peer_addr(b_full, 0) : b_full;
-      const bool a_mn = g.a_mn, b_mn = g.b_mn;
-      const uint32_t nkb0 = g.nkb[0], stage_bytes = g.stage_bytes;
-      for (Tiles<EPI, CG> ts(g, wn); ts.more(); ts.next()) {
-        const Tile ti = ts.at();
-        const int am = (int)(ti.m0 + rank * BM);
-        // a 512-column tile is two products of 256: this CTA's half of each
-        const uint32_t half_b = g.bn > 256 ? 128u : bl;
-        const int bn0 = (int)(TWO && g.bn <= 256 ? ti.n0 : ti.n0 + rank * half_b);
-        const uint32_t e = kb_last(ti);
-        uint32_t kb = kb_first(ti);
-        // dw: the batch's A; else the segment's A and B
-        const CUtensorMap* ma = &maps.a[EPI == EPI_PARTIAL ? ti.batch : 0];
-        const CUtensorMap* mb = &maps.b[TWO && CG == 2 && g.bn <= 256 ? rank : 0];  // a weight a CTA
-        int k0 = (int)kb * kw;
-        for (; kb < e; kb++, k0 += kw) {
-          if (EPI != EPI_PARTIAL && !TWO && kb == nkb0) {  // the second segment
-            ma = &maps.a[1];
-            mb = &maps.b[1];
-            k0 = 0;
-          }
-          if (!mbar_wait(b_empty + 8 * s, ph ^ 1u, abort_flag, g.err, 70)) goto drain;
-          if (rank == 0) mbar_expect_tx(b_full + 8 * s, tx);
-          const uint32_t bar = b_land + 8 * s;
-          if (a_mn) {
-#pragma unroll
-            for (int i = 0; i < BM / 64; i++)
-              tma_load_2d<CG>(st + i * 8192, ma, am + i * 64, k0, bar);
-          } else {
-            tma_load_2d<CG>(st, ma, k0, am, bar);
-          }
-          if (b_mn) {
-            for (uint32_t i = 0; i < bl; i += 64)
-              tma_load_2d<CG>(st + A_BYTES + i * 128, mb,
-                              bn0 + (int)(i < half_b ? i : i + 128), k0, bar);
-          } else if (g.bn > 256) {
-            tma_load_2d<CG>(st + A_BYTES, mb, k0, bn0, bar);
-            tma_load_2d<CG>(st + A_BYTES + 128 * 128, TWO ? &maps.b[1] : mb, k0,
-                            TWO ? bn0 : bn0 + 256, bar);
-          } else {
-            tma_load_2d<CG>(st + A_BYTES, mb, k0, bn0, bar);
-            if (TWO && CG == 1)
-              tma_load_2d<CG>(st + A_BYTES + wn * 128, &maps.b[1], k0, bn0, bar);
-          }
-          filled++;
-          st += stage_bytes;
-          if (++s == S) s = 0, ph ^= 1u, st = base;
-        }
-      }
-    drain:
-      if (*abort_flag && rank == 0)  // the last fill of every stage lands before the CTA ends
-        for (uint64_t f = filled > S ? filled - S : 0; f < filled; f++)
-          mbar_drain(b_full + 8 * (uint32_t)(f % S), (uint32_t)((f / S) & 1u));
-    }
-  } else if (warp == EPI_WARPS + 1) {
-    // ---- MMA issuer ----
-    if (lane == 0 && rank == 0) {
-      uint32_t s = 0, ph = 0, buf = 0, aph = 0;
-      // The issuing thread's own instructions bound a stage once (about 1000
-      // clocks against 512 of products): the descriptors are one addition each.
-      const uint64_t desc_a = smem_desc(base, g.a_mn), desc_b = smem_desc(base + A_BYTES, g.b_mn);
-      const uint32_t step_a = (g.a_mn ? 2048u : 32u) >> 4, step_b = (g.b_mn ? 2048u : 32u) >> 4;
-      const uint32_t stage16 = g.stage_bytes >> 4, idesc = g.idesc, bn = g.bn;
-      auto issue = [&](auto fp8, auto wide) -> bool {
+    if (warp == EPI_WARPS) {
+      // ---- TMA producer ----
+      if (lane == 0) {
+        uint32_t s = 0, ph = 0, st = base;
+        uint64_t filled = 0;
+        const uint32_t tx = CG * (A_BYTES + bl * 128);
+        const int kw = g.fp8 ? 128 : 64;  // elements of a k block
+        // both CTAs' loads count on the issuing CTA's barriers
+        const uint32_t b_land = CG == 2 ? peer_addr(b_full, 0) : b_full;
+        const bool a_mn = g.a_mn, b_mn = g.b_mn;
+        const uint32_t nkb0 = g.nkb[0], stage_bytes = g.stage_bytes;
         for (Tiles<EPI, CG> ts(g, wn); ts.more(); ts.next()) {
           const Tile ti = ts.at();
-          const uint32_t last = kb_last(ti);
+          const int am = (int)(ti.m0 + rank * BM);
+          // a 512-column tile is two products of 256: this CTA's half of each
+          const uint32_t half_b = g.bn > 256 ? 128u : bl;
+          const int bn0 = (int)(TWO && g.bn <= 256 ? ti.n0 : ti.n0 + rank * half_b);
+          const uint32_t e = kb_last(ti);
           uint32_t kb = kb_first(ti);
-          do {  // a piece of the contraction into one accumulator
-            const uint32_t e = EPI == EPI_LINEAR_F32 && last - kb > PIECE ? kb + PIECE : last;
-            if (!mbar_wait(b_acce + 8 * buf, aph ^ 1u, abort_flag, g.err, 71)) return false;
-            tc_fence_after();
-            const uint32_t d = tmem + buf * bn;
-            uint32_t acc = 0u;
-            for (; kb < e; kb++) {
-              if (!mbar_wait(b_full + 8 * s, ph, abort_flag, g.err, 72)) return false;
-              tc_fence_after();
-              const uint64_t da = desc_a + s * stage16, db = desc_b + s * stage16;
-#pragma unroll
-              for (uint32_t kk = 0; kk < 4; kk++) {
-                if (decltype(fp8)::value) mma_f8<CG>(d, da + kk * step_a, db + kk * step_b, idesc, acc);
-                else mma_f16<CG>(d, da + kk * step_a, db + kk * step_b, idesc, acc);
-                if (decltype(wide)::value) {  // the second 256 columns; A stays where it is
-                  const uint64_t d2 = db + (128 * 128 >> 4) + kk * step_b;
-                  if (decltype(fp8)::value) mma_f8<CG>(d + 256, da + kk * step_a, d2, idesc, acc);
-                  else mma_f16<CG>(d + 256, da + kk * step_a, d2, idesc, acc);
-                }
-                acc = 1u;
-              }
-              mma_commit<CG>(b_empty + 8 * s);
-              if (++s == S) s = 0, ph ^= 1u;
+          // dw: the batch's A; else the segment's A and B
+          const CUtensorMap* ma = &maps.a[EPI == EPI_PARTIAL ? ti.batch : 0];
+          const CUtensorMap* mb = &maps.b[TWO && CG == 2 && g.bn <= 256 ? rank : 0];  // a weight a CTA
+          int k0 = (int)kb * kw;
+          for (; kb < e; kb++, k0 += kw) {
+            if (EPI != EPI_PARTIAL && !TWO && kb == nkb0) {  // the second segment
+              ma = &maps.a[1];
+              mb = &maps.b[1];
+              k0 = 0;
             }
-            mma_commit<CG>(b_accf + 8 * buf);
-            if (++buf == bufs) buf = 0, aph ^= 1u;
-          } while (kb < last);
+            if (!mbar_wait(b_empty + 8 * s, ph ^ 1u, abort_flag, g.err, 70)) goto drain;
+            if (rank == 0) mbar_expect_tx(b_full + 8 * s, tx);
+            const uint32_t bar = b_land + 8 * s;
+            if (a_mn) {
+#pragma unroll
+              for (int i = 0; i < BM / 64; i++)
+                tma_load_2d<CG>(st + i * 8192, ma, am + i * 64, k0, bar);
+            } else {
+              tma_load_2d<CG>(st, ma, k0, am, bar);
+            }
+            if (b_mn) {
+              for (uint32_t i = 0; i < bl; i += 64)
+                tma_load_2d<CG>(st + A_BYTES + i * 128, mb,
+                                bn0 + (int)(i < half_b ? i : i + 128), k0, bar);
+            } else if (g.bn > 256) {
+              tma_load_2d<CG>(st + A_BYTES, mb, k0, bn0, bar);
+              tma_load_2d<CG>(st + A_BYTES + 128 * 128, TWO ? &maps.b[1] : mb, k0,
+                              TWO ? bn0 : bn0 + 256, bar);
+            } else {
+              tma_load_2d<CG>(st + A_BYTES, mb, k0, bn0, bar);
+              if (TWO && CG == 1)
+                tma_load_2d<CG>(st + A_BYTES + wn * 128, &maps.b[1], k0, bn0, bar);
+            }
+            filled++;
+            st += stage_bytes;
+            if (++s == S) s = 0, ph ^= 1u, st = base;
+          }
         }
-        return true;
-      };
-      if (CG == 2 && bufs == 1) {
-        if (g.fp8) issue(std::true_type{}, std::true_type{});
-        else issue(std::false_type{}, std::true_type{});
-      } else {
-        if (g.fp8) issue(std::true_type{}, std::false_type{});
-        else issue(std::false_type{}, std::false_type{});
+      drain:
+        if (*abort_flag && rank == 0)  // the last fill of every stage lands before the CTA ends
+          for (uint64_t f = filled > S ? filled - S : 0; f < filled; f++)
+            mbar_drain(b_full + 8 * (uint32_t)(f % S), (uint32_t)((f / S) & 1u));
       }
-      // every product issued is done before tensor memory is freed
-      mma_commit_here<CG>(b_last);
-      mbar_drain(b_last, 0);
+    } else if (warp == EPI_WARPS + 1) {
+      // ---- MMA issuer ----
+      if (lane == 0 && rank == 0) {
+        uint32_t s = 0, ph = 0, buf = 0, aph = 0;
+        // The issuing thread's own instructions bound a stage once (about 1000
+        // clocks against 512 of products): the descriptors are one addition each.
+        const uint64_t desc_a = smem_desc(base, g.a_mn), desc_b = smem_desc(base + A_BYTES, g.b_mn);
+        const uint32_t step_a = (g.a_mn ? 2048u : 32u) >> 4, step_b = (g.b_mn ? 2048u : 32u) >> 4;
+        const uint32_t stage16 = g.stage_bytes >> 4, idesc = g.idesc, bn = g.bn;
+        auto issue = [&](auto fp8, auto wide) -> bool {
+          for (Tiles<EPI, CG> ts(g, wn); ts.more(); ts.next()) {
+            const Tile ti = ts.at();
+            const uint32_t last = kb_last(ti);
+            uint32_t kb = kb_first(ti);
+            do {  // a piece of the contraction into one accumulator
+              const uint32_t e = EPI == EPI_LINEAR_F32 && last - kb > PIECE ? kb + PIECE : last;
+              if (!mbar_wait(b_acce + 8 * buf, aph ^ 1u, abort_flag, g.err, 71)) return false;
+              tc_fence_after();
+              const uint32_t d = tmem + buf * bn;
+              uint32_t acc = 0u;
+              for (; kb < e; kb++) {
+                if (!mbar_wait(b_full + 8 * s, ph, abort_flag, g.err, 72)) return false;
+                tc_fence_after();
+                const uint64_t da = desc_a + s * stage16, db = desc_b + s * stage16;
+#pragma unroll
+                for (uint32_t kk = 0; kk < 4; kk++) {
+                  if (decltype(fp8)::value) mma_f8<CG>(d, da + kk * step_a, db + kk * step_b, idesc, acc);
+                  else mma_f16<CG>(d, da + kk * step_a, db + kk * step_b, idesc, acc);
+                  if (decltype(wide)::value) {  // the second 256 columns; A stays where it is
+                    const uint64_t d2 = db + (128 * 128 >> 4) + kk * step_b;
+                    if (decltype(fp8)::value) mma_f8<CG>(d + 256, da + kk * step_a, d2, idesc, acc);
+                    else mma_f16<CG>(d + 256, da + kk * step_a, d2, idesc, acc);
+                  }
+                  acc = 1u;
+                }
+                mma_commit<CG>(b_empty + 8 * s);
+                if (++s == S) s = 0, ph ^= 1u;
+              }
+              mma_commit<CG>(b_accf + 8 * buf);
+              if (++buf == bufs) buf = 0, aph ^= 1u;
+            } while (kb < last);
+          }
+          return true;
+        };
+        if (CG == 2 && bufs == 1) {
+          if (g.fp8) issue(std::true_type{}, std::true_type{});
+          else issue(std::false_type{}, std::true_type{});
+        } else {
+          if (g.fp8) issue(std::true_type{}, std::false_type{});
+          else issue(std::false_type{}, std::false_type{});
+        }
+        // every product issued is done before tensor memory is freed
+        mma_commit_here<CG>(b_last);
+        mbar_drain(b_last, 0);
+      }
     }
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(EPI_REGS));
     // ---- epilogue ----
@@ -1043,7 +1051,8 @@ int make_chunk_map(bgnn_ctx* ctx, CUtensorMap* map, int type, const Mat& x) {
                                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   const CUresult r =
       enc(map, dt, 2, const_cast<void*>(x.p), dims, strides, box, el,
-          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+          CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return bgnn_set_error(ctx, BGNN_ERR_UNSUPPORTED, "tensor map encode failed (%d)", (int)r);
   return BGNN_OK;

@@ -744,7 +744,11 @@ extern "C" int bgnn_rms_norm(bgnn_ctx* ctx, int x_type, const void* x, uint64_t 
   BGNN_REQUIRE(ctx, !residual || res_type == x_type || res_type == BGNN_F32,
                "rms_norm: the residual has the input's type or f32");
   BGNN_REQUIRE(ctx, eps >= 0.0, "rms_norm: negative or NaN eps");
-  if (rows == 0 || cols == 0) return BGNN_OK;
+  if (rows == 0 || cols == 0) {
+    if (rows && scale && out_type == BGNN_E4M3)
+      BGNN_CUDA(ctx, cudaMemsetAsync(scale, 0, rows * sizeof(float), ctx->stream));
+    return BGNN_OK;
+  }
   BGNN_REQUIRE(ctx, x && weight && out, "rms_norm: NULL argument");
   BGNN_REQUIRE(ctx, !residual || total, "rms_norm: a residual needs a buffer for the sum");
   BGNN_REQUIRE(ctx, out_type != BGNN_E4M3 || scale, "rms_norm: an e4m3 output needs scales");

@@ -564,7 +564,7 @@ BGNN_API int bgnn_link_scores(bgnn_ctx* ctx, const float* emb, uint32_t num_node
  *       residual's own buffer when ld_res == cols)
  *   y = t * (mean(t^2) + eps)^(-1/2) * weight
  *   out = y, or for BGNN_E4M3 y / scale[row] with scale = max|y| / 448 (1 for
- *       an all-zero row; e4m3 rounds to nearest even).
+ *       an all-zero row, 0 without columns; e4m3 rounds to nearest even).
  * x f32, bf16 or f16; the residual has x's type or f32; weight [cols] any of
  * the three; out f32, bf16, f16 or e4m3 (scale [rows], else NULL).  A row that
  * holds a NaN or an infinity gives NaN in what it touches, and a NaN scale or

@@ -111,6 +111,9 @@ def test_rms_norm_one_row_and_empty():
     assert a.shape == (64,) and total.shape == (64,) and torch.equal(a, b[0])
     out, total, scale = bg.rmsNorm(torch.empty(0, 64, device="cuda"), w, outType=F8)
     assert out.shape == (0, 64) and scale.shape == (0,)
+    none = torch.empty(3, 0, device="cuda")
+    out, _, scale = bg.rmsNorm(none, torch.empty(0, device="cuda"), outType=F8)
+    assert out.shape == (3, 0) and (scale == 0).all()
     gx, gw = bg.rmsNormBackward(torch.empty(0, 64, device="cuda"),
                                 torch.empty(0, 64, device="cuda"), w)
     assert gx.shape == (0, 64) and torch.equal(gw, torch.zeros_like(w))
