@@ -41,10 +41,11 @@ class CudaContext:
         self.device = int(device)
         self._stream = None
         self._math = _lib.MATH_FAST
+        # current_stream(device).cuda_stream without building a Stream object
+        self._raw_stream = torch._C._cuda_getCurrentRawStream
 
     def bind(self):
-        # current_stream(device).cuda_stream without building a Stream object
-        s = _torch()._C._cuda_getCurrentRawStream(self.device)
+        s = self._raw_stream(self.device)
         if s != self._stream:
             _lib.check(self.lib.bgnn_ctx_set_stream(self.h, s if s else None), self.h)
             self._stream = s
@@ -100,6 +101,9 @@ _contexts: dict = {}
 
 
 def get_context(device: Optional[int] = None) -> CudaContext:
+    ctx = _contexts.get(device)
+    if ctx is not None:
+        return ctx
     torch = _torch()
     if device is None:
         device = torch.cuda.current_device() if torch.cuda.is_available() else 0

@@ -101,18 +101,18 @@ def _rows(t, name):
     """[rows, cols] with unit column stride and rows that do not overlap, and
     whether the tensor was one row."""
     _tensor(t, name)
-    one = t.dim() == 1
-    if one:
+    dim = t.dim()
+    if dim == 1:
         t = t.unsqueeze(0)
-    elif t.dim() != 2:
-        raise ValueError(f"{name}: expects 1D or 2D input, got {t.dim()}D")
-    if not t.is_contiguous():
-        rows, cols = t.shape
-        if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
-            t = t.contiguous()
-    if t.shape[1] >= 2 ** 31:
-        raise ValueError(f"{name}: a row of {t.shape[1]} elements")
-    return t, one
+    elif dim != 2:
+        raise ValueError(f"{name}: expects 1D or 2D input, got {dim}D")
+    rows, cols = t.shape
+    if not t.is_contiguous() and ((cols > 1 and t.stride(1) != 1) or
+                                  (rows > 1 and t.stride(0) < cols)):
+        t = t.contiguous()
+    if cols >= 2 ** 31:
+        raise ValueError(f"{name}: a row of {cols} elements")
+    return t, dim == 1
 
 
 def _ld(t):
@@ -128,7 +128,7 @@ def _vec(t, n, name, allowed):
     _tensor(t, name)
     if t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{name}: expected shape [{n}], got {list(t.shape)}")
-    return t.contiguous(), _type(t.dtype, name, allowed)
+    return t if t.is_contiguous() else t.contiguous(), _type(t.dtype, name, allowed)
 
 
 def _same_shape(t, rows, cols, name):
