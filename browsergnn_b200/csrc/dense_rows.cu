@@ -138,25 +138,30 @@ __global__ void __launch_bounds__(WARPS * 32) k_dense_rows(const RowsArgs a) {
   store_any(a.out, a.out_type, row * a.ld_out + col, o);
 }
 
-template <int DT, int M, bool TWO>
-int launch_vec(bgnn_ctx* ctx, const RowsArgs& a, bool vec) {
+template <int DT, int M, bool TWO, int VEC>
+int launch_rows(bgnn_ctx* ctx, const RowsArgs& a) {
   const dim3 grid((a.n + WARPS - 1) / WARPS, (a.m + M - 1) / M);
-  constexpr int VEC = DT == BGNN_E4M3 ? 16 : 8;
-  if (vec) k_dense_rows<DT, M, TWO, VEC><<<grid, WARPS * 32, 0, ctx->stream>>>(a);
-  else k_dense_rows<DT, M, TWO, 1><<<grid, WARPS * 32, 0, ctx->stream>>>(a);
+  k_dense_rows<DT, M, TWO, VEC><<<grid, WARPS * 32, 0, ctx->stream>>>(a);
   BGNN_LAUNCHED(ctx);
   return BGNN_OK;
 }
+// Single elements go four rows at a time at most: with eight, 8 x 3,501 -> 3,901
+// takes 109 us against 35, and 100 x 301 -> 271 takes 11.3 against 5.6.
+template <int DT, bool TWO, int VEC>
+int launch_m(bgnn_ctx* ctx, const RowsArgs& a) {
+  if (a.m == 1) return launch_rows<DT, 1, TWO, VEC>(ctx, a);
+  if (a.m == 2) return launch_rows<DT, 2, TWO, VEC>(ctx, a);
+  if (a.m <= 4 || VEC == 1) return launch_rows<DT, 4, TWO, VEC>(ctx, a);
+  return launch_rows<DT, VEC == 1 ? 4 : 8, TWO, VEC>(ctx, a);
+}
 template <int DT, bool TWO>
-int launch_m(bgnn_ctx* ctx, const RowsArgs& a, bool vec) {
-  if (a.m == 1) return launch_vec<DT, 1, TWO>(ctx, a, vec);
-  if (a.m == 2) return launch_vec<DT, 2, TWO>(ctx, a, vec);
-  if (a.m <= 4) return launch_vec<DT, 4, TWO>(ctx, a, vec);
-  return launch_vec<DT, 8, TWO>(ctx, a, vec);
+int launch_vec(bgnn_ctx* ctx, const RowsArgs& a, bool vec) {
+  constexpr int VEC = DT == BGNN_E4M3 ? 16 : 8;
+  return vec ? launch_m<DT, TWO, VEC>(ctx, a) : launch_m<DT, TWO, 1>(ctx, a);
 }
 template <int DT>
 int launch_two(bgnn_ctx* ctx, const RowsArgs& a, bool vec) {
-  return a.two ? launch_m<DT, true>(ctx, a, vec) : launch_m<DT, false>(ctx, a, vec);
+  return a.two ? launch_vec<DT, true>(ctx, a, vec) : launch_vec<DT, false>(ctx, a, vec);
 }
 
 }  // namespace

@@ -233,6 +233,7 @@ PRODUCTS = [  # m, k, n, type, act, bias, residual, out
     (1001, 40, 32, BF, "silu", BF, F32, F32), (1025, 40, 32, BF, "silu", BF, F32, F32),
     (21, 9000, 88, F16, None, None, None, F32), (21, 9100, 88, F16, None, None, None, F32),
     (700, 130, 120, F8, "gelu", BF, BF, BF),
+    (5, 3501, 2700, BF, None, None, None, BF), (7, 301, 271, F8, "silu", BF, None, BF),
 ]
 
 
