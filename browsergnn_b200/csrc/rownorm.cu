@@ -24,6 +24,7 @@
 // registers of a block hold (RowShape) take the k_*_long kernels, which read
 // the row again from L2.
 #include "lowp.cuh"
+#include "row_words.cuh"
 
 namespace {
 
@@ -37,6 +38,7 @@ struct RmsArgs {
   uint64_t rows;
   uint32_t cols;
   float eps;
+  uint32_t edge;  // edge_rows of the operands
   void* total;
   void* out;
   float* scale;
@@ -136,7 +138,8 @@ struct Words {
   static constexpr int W = 8 / PER;
   uint4 w[NV][W + MIS];
   uint32_t sh;
-  // vector i is columns [c0 + i * step, + 8); none from cols on
+  // vector i is columns [c0 + i * step, + 8); none from cols on.  Its words are
+  // read whole: of inner rows only, or with !MIS, where they are the vector's.
   __device__ __forceinline__ void fetch(const elt_t<DT>* row, uint32_t c0, uint32_t step,
                                         uint32_t cols) {
     const char* p = reinterpret_cast<const char*>(row + c0);
@@ -149,7 +152,7 @@ struct Words {
         w[i][k] = c0 + i * step < cols ? q[k] : make_uint4(0, 0, 0, 0);
     }
   }
-  // the first and the last row: no word reaches out of the matrix
+  // the first and the last rows (edge_rows): no word reaches out of the matrix
   __device__ __forceinline__ void fetch_edge(const elt_t<DT>* row, uint32_t c0, uint32_t step,
                                              uint32_t cols, const Span& m) {
     const char* p = reinterpret_cast<const char*>(row + c0);
@@ -281,7 +284,7 @@ __global__ void __launch_bounds__(NV == 1 ? 256 : 512, NV > 1 ? 1 : MIS ? 4 : 5)
   for (uint64_t base = (uint64_t)blockIdx.x * at.rpb; base < a.rows;
        base += (uint64_t)gridDim.x * at.rpb) {
     const uint64_t row = base + at.sub;
-    const bool on = row < a.rows, inner = row != 0 && row + 1 < a.rows;
+    const bool on = row < a.rows, inner = inner_row(row, a.rows, a.edge);
     const uint32_t cols = on ? a.cols : 0;
     const uint32_t c0 = at.first + at.lane * 8, step = at.lanes * 8;
     float t[NV][8];
@@ -415,6 +418,7 @@ struct RmsBwdArgs {
   uint64_t rows;
   uint32_t cols;
   float eps;
+  uint32_t edge;  // edge_rows of the operands
   void* gx;
   float* part;  // [grid, cols] sums of gy * xh over each block's rows
 };
@@ -449,7 +453,7 @@ __global__ void __launch_bounds__(512) k_rms_bwd(const RmsBwdArgs a, int tpr,
   for (uint64_t base = (uint64_t)blockIdx.x * at.rpb; base < a.rows;
        base += (uint64_t)gridDim.x * at.rpb) {
     const uint64_t row = base + at.sub;
-    const bool on = row < a.rows, inner = row != 0 && row + 1 < a.rows;
+    const bool on = row < a.rows, inner = inner_row(row, a.rows, a.edge);
     const uint32_t cols = on ? a.cols : 0;
     const elt_t<TT>* sr = static_cast<const elt_t<TT>*>(a.gt) + row * a.ld_gt;
     // the row stays as stored (16-bit: half the registers) and is unpacked twice
@@ -764,6 +768,7 @@ extern "C" int bgnn_rms_norm(bgnn_ctx* ctx, int x_type, const void* x, uint64_t 
   a.rows = rows;
   a.cols = cols;
   a.eps = (float)eps;
+  a.edge = edge_rows(residual && ld_res < ld_x ? ld_res : ld_x);
   a.total = total;
   a.out = out;
   a.scale = scale;
@@ -818,6 +823,9 @@ extern "C" int bgnn_rms_norm_backward(bgnn_ctx* ctx, int grad_type, const void* 
   a.rows = rows;
   a.cols = cols;
   a.eps = (float)eps;
+  uint64_t ld = ld_grad < ld_total ? ld_grad : ld_total;
+  if (grad_total && ld_grad_total < ld) ld = ld_grad_total;
+  a.edge = edge_rows(ld);
   a.gx = grad_x;
   a.part = nullptr;
   const bool vec = cols % 8 == 0 && vec_rows(grad, ld_grad) && vec_rows(total, ld_total) &&
