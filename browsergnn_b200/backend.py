@@ -12,6 +12,7 @@ raises, and the backend refuses to initialise without a CUDA device.
 from __future__ import annotations
 
 import ctypes
+import threading
 from typing import Optional
 
 import numpy as np
@@ -28,7 +29,12 @@ def _torch():
 
 
 class CudaContext:
-    """One libbgnn context per device, following torch's current stream."""
+    """One libbgnn context per device, following torch's current stream.
+
+    A library context serves one host thread at a time, and its stream is set
+    before each call: `lock` is held over both (and over the reading of the
+    call's error), so that threads with streams of their own may share the
+    context.  Re-entrant, because a graph's finaliser may run inside a call."""
 
     def __init__(self, device: int = 0):
         torch = _torch()
@@ -43,8 +49,10 @@ class CudaContext:
         self._math = _lib.MATH_FAST
         # current_stream(device).cuda_stream without building a Stream object
         self._raw_stream = torch._C._cuda_getCurrentRawStream
+        self.lock = threading.RLock()
 
     def bind(self):
+        """Sets the library's stream; a call that relies on it holds `lock`."""
         s = self._raw_stream(self.device)
         if s != self._stream:
             _lib.check(self.lib.bgnn_ctx_set_stream(self.h, s if s else None), self.h)
@@ -52,16 +60,19 @@ class CudaContext:
         return self.h
 
     def call(self, name: str, *args):
-        h = self.bind()
-        rc = getattr(self.lib, name)(h, *args)
-        _lib.check(rc, self.h)
+        with self.lock:
+            h = self.bind()
+            rc = getattr(self.lib, name)(h, *args)
+            if rc:
+                _lib.check(rc, self.h)
 
     def call_on(self, name: str, *args):
         """Call an entry point whose first argument is another handle (a
         partition, a communicator) that reports errors on this context."""
-        self.bind()
-        rc = getattr(self.lib, name)(*args)
-        _lib.check(rc, self.h)
+        with self.lock:
+            self.bind()
+            rc = getattr(self.lib, name)(*args)
+            _lib.check(rc, self.h)
 
     def set_math(self, mode):
         """True / "exact": the reference's rounding, bit for bit; False /
@@ -76,16 +87,18 @@ class CudaContext:
             code = _lib.MATH_TENSOR
         else:
             raise ValueError(f"unknown math mode {mode!r}")
-        _lib.check(self.lib.bgnn_ctx_set_math(self.h, code), self.h)
-        self._math = code
+        with self.lock:
+            _lib.check(self.lib.bgnn_ctx_set_math(self.h, code), self.h)
+            self._math = code
 
     @property
     def exact(self) -> bool:
         return self._math == _lib.MATH_EXACT
 
     def synchronize(self):
-        self.bind()
-        _lib.check(self.lib.bgnn_ctx_synchronize(self.h), self.h)
+        with self.lock:
+            self.bind()
+            _lib.check(self.lib.bgnn_ctx_synchronize(self.h), self.h)
 
     @property
     def launches(self) -> int:
@@ -98,6 +111,7 @@ class CudaContext:
 
 
 _contexts: dict = {}
+_contexts_lock = threading.Lock()
 
 
 def get_context(device: Optional[int] = None) -> CudaContext:
@@ -107,10 +121,11 @@ def get_context(device: Optional[int] = None) -> CudaContext:
     torch = _torch()
     if device is None:
         device = torch.cuda.current_device() if torch.cuda.is_available() else 0
-    ctx = _contexts.get(device)
-    if ctx is None:
-        ctx = CudaContext(device)
-        _contexts[device] = ctx
+    with _contexts_lock:
+        ctx = _contexts.get(device)
+        if ctx is None:
+            ctx = CudaContext(device)
+            _contexts[device] = ctx
     return ctx
 
 

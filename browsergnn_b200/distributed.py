@@ -94,13 +94,11 @@ class DistContext:
 
     def allreduce_max(self, values: Sequence[float]) -> List[float]:
         arr = (ctypes.c_double * len(values))(*[float(v) for v in values])
-        self.ctx.bind()
-        _lib.check(self.ctx.lib.bgnn_dist_allreduce_max(self.h, arr, len(values)), self.ctx.h)
+        self.ctx.call_on("bgnn_dist_allreduce_max", self.h, arr, len(values))
         return list(arr)
 
     def synchronize(self):
-        self.ctx.bind()
-        _lib.check(self.ctx.lib.bgnn_dist_synchronize(self.h), self.ctx.h)
+        self.ctx.call_on("bgnn_dist_synchronize", self.h)
 
     def abort(self):
         """Abort the communicator after learning on the host that a peer is
