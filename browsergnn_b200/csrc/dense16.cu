@@ -141,7 +141,7 @@ __device__ __forceinline__ bool mbar_try(uint32_t a, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// bounded wait; false when it gave up or another role already did
+// bounded wait of one thread; false when it gave up or another role already did
 __device__ __forceinline__ bool mbar_wait(uint32_t a, uint32_t parity, volatile uint32_t* abort_flag,
                                           int* err, int where) {
   long long t0 = 0;
@@ -156,6 +156,14 @@ __device__ __forceinline__ bool mbar_wait(uint32_t a, uint32_t parity, volatile 
   *abort_flag = 1u;
   dev_raise(err, DEVERR_TIMEOUT, (uint64_t)blockIdx.x, where);
   return false;
+}
+// The same for a whole warp.  Each lane polls (what it reads next is ordered
+// after its own wait), and one that gave up takes the others along: the warp's
+// next instructions need all of its lanes, and lanes that left alone would keep
+// the rest waiting there without a limit.
+__device__ __forceinline__ bool warp_wait(uint32_t a, uint32_t parity, volatile uint32_t* abort_flag,
+                                          int* err, int where) {
+  return __all_sync(0xffffffffu, mbar_wait(a, parity, abort_flag, err, where)) != 0;
 }
 // for what is in flight when a role has given up
 __device__ __forceinline__ void mbar_drain(uint32_t a, uint32_t parity) {
@@ -207,6 +215,7 @@ template <int CG>
 __device__ __forceinline__ void pair_sync() {
   __syncthreads();
   if constexpr (CG == 2) {
+    __syncwarp();  // one lane of a warp may have come another way
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
@@ -648,7 +657,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       };
       auto asked = [&]() {
-        if (!mbar_wait(in_bar, in_ph, abort_flag, g.err, 74)) {
+        if (!warp_wait(in_bar, in_ph, abort_flag, g.err, 74)) {
           gave_up = true;
           mbar_drain(in_bar, in_ph);
         }
@@ -781,7 +790,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int j = 0; j < 32; j++) sum[i][j] = 0.0f;
         uint32_t kb = k_first;
         do {
-          if (!mbar_wait(b_accf + 8 * buf, aph, abort_flag, g.err, 73)) {
+          if (!warp_wait(b_accf + 8 * buf, aph, abort_flag, g.err, 73)) {
             gave_up = true;
             break;
           }
@@ -811,7 +820,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
         }
       } else {
-        if (!mbar_wait(b_accf + 8 * buf, aph, abort_flag, g.err, 73)) break;
+        if (!warp_wait(b_accf + 8 * buf, aph, abort_flag, g.err, 73)) break;
         tc_fence_after();
         const uint32_t acc = tmem + lanes + buf * g.bn;
         for (uint32_t c = group * 32; c < wn; c += 128) {
@@ -905,6 +914,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   pair_sync<CG>();
   if (warp == EPI_WARPS) {
+    __syncwarp();
     tc_fence_after();
     tmem_free<CG>(tmem, tmem_cols);
   }
