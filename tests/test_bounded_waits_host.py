@@ -16,10 +16,10 @@ def epilogue(name):
     return text, re.split(r"\n}\n", parts[1])[0]
 
 
-@pytest.mark.parametrize("name", ["dense16.cu"])
+@pytest.mark.parametrize("name", ["dense16.cu", "gemm_tc.cu"])
 def test_a_warp_gives_up_as_one(name):
     text, body = epilogue(name)
     assert body.count("warp_wait(") >= 1
     assert not re.search(r"\bmbar_wait\(", body)
     helper = re.search(r"bool warp_wait\(.*?\n}\n", text, re.S).group(0)
-    assert "__all_sync(0xffffffffu, mbar_wait(" in helper
+    assert re.search(r"__all_sync\(0xffffffffu, mbar_(wait|try)\(", helper)
