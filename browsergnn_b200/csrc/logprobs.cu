@@ -749,6 +749,7 @@ extern "C" int bgnn_log_probs(bgnn_ctx* ctx, int type, const void* logits, uint6
                               float* lse, uint32_t* top_ids, float* top_logp) {
   BGNN_ON_DEVICE(ctx);
   BGNN_REQUIRE(ctx, dtype_float(type), "log_probs: unknown element type %d", type);
+  BGNN_REQUIRE_COLS(ctx, "log_probs", cols);
   BGNN_REQUIRE(ctx, top_k <= TOP_MAX, "log_probs: top_k %u above %d", top_k, TOP_MAX);
   if (rows == 0) return BGNN_OK;
   BGNN_REQUIRE(ctx, logits || cols == 0, "log_probs: NULL logits");
@@ -785,6 +786,7 @@ extern "C" int bgnn_log_probs_backward(bgnn_ctx* ctx, int type, const void* logi
                                        const float* grad_entropy, void* grad_logits) {
   BGNN_ON_DEVICE(ctx);
   BGNN_REQUIRE(ctx, dtype_float(type), "log_probs_backward: unknown element type %d", type);
+  BGNN_REQUIRE_COLS(ctx, "log_probs_backward", cols);
   if (rows == 0 || cols == 0) return BGNN_OK;
   BGNN_REQUIRE(ctx, logits && targets && lse && grad_logits, "log_probs_backward: NULL argument");
   BGNN_REQUIRE(ctx, !grad_entropy || entropy, "log_probs_backward: grad_entropy needs the entropy");

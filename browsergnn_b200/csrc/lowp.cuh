@@ -40,6 +40,10 @@ struct DeviceGuard {
   DeviceGuard device_guard_(ctx); \
   if (device_guard_.status != BGNN_OK) return device_guard_.status
 
+// Columns of a row are counted in 32 bits with room for a block's step.
+#define BGNN_REQUIRE_COLS(ctx, name, cols) \
+  BGNN_REQUIRE(ctx, (cols) <= 0x7fffffffu, "%s: a row of %u elements, 2^31 or more", name, cols)
+
 // out[c] = the sum of column c over `parts` rows of f32 partial sums, in a
 // fixed order (rownorm.cu)
 int bgnn_run_sum_parts(bgnn_ctx* ctx, const float* part, uint32_t parts, uint64_t cols, void* out,

@@ -747,6 +747,7 @@ extern "C" int bgnn_rms_norm(bgnn_ctx* ctx, int x_type, const void* x, uint64_t 
                "rms_norm: unknown output type %d", out_type);
   BGNN_REQUIRE(ctx, !residual || res_type == x_type || res_type == BGNN_F32,
                "rms_norm: the residual has the input's type or f32");
+  BGNN_REQUIRE_COLS(ctx, "rms_norm", cols);
   BGNN_REQUIRE(ctx, eps >= 0.0, "rms_norm: negative or NaN eps");
   if (rows == 0 || cols == 0) {
     if (rows && scale && out_type == BGNN_E4M3)
@@ -801,6 +802,7 @@ extern "C" int bgnn_rms_norm_backward(bgnn_ctx* ctx, int grad_type, const void* 
                "rms_norm_backward: unknown element type");
   BGNN_REQUIRE(ctx, grad_type == total_type || total_type == BGNN_F32,
                "rms_norm_backward: the gradient has the row's type, or the row is f32");
+  BGNN_REQUIRE_COLS(ctx, "rms_norm_backward", cols);
   BGNN_REQUIRE(ctx, eps >= 0.0, "rms_norm_backward: negative or NaN eps");
   if (cols == 0) return BGNN_OK;
   if (rows == 0) {

@@ -555,8 +555,8 @@ BGNN_API int bgnn_link_scores(bgnn_ctx* ctx, const float* emb, uint32_t num_node
  * operands.  Types are bgnn_dtype; device pointers, asynchronous on the
  * context's stream; row strides (ld_*) count elements and are at least the
  * row length; outputs without a stride are contiguous; inputs and outputs do
- * not overlap unless said.  Sums, statistics and epilogues are f32 and every
- * output is rounded once. */
+ * not overlap unless said.  Rows hold fewer than 2^31 elements.  Sums,
+ * statistics and epilogues are f32 and every output is rounded once. */
 
 /* Root-mean-square norm with the residual's addition:
  *   t = x + residual, rounded to the residual's type -> total [rows, cols]
