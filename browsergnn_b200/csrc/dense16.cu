@@ -1406,6 +1406,8 @@ extern "C" int bgnn_linear_fused(bgnn_ctx* ctx, int type, const void* x, uint64_
                "linear_fused: residual type or row stride");
   if (m == 0 || n == 0) return BGNN_OK;
   BGNN_REQUIRE(ctx, out && ld_out >= n, "linear_fused: NULL out or its row stride below n");
+  BGNN_REQUIRE(ctx, residual != out || (res_type == out_type && (m == 1 || ld_res == ld_out)),
+               "linear_fused: out in the residual's buffer needs its type and row stride");
   BGNN_REQUIRE(ctx, type != BGNN_E4M3 || (x_scale && w_scale),
                "linear_fused: e4m3 operands need a scale a row");
   GemmArgs g = {};

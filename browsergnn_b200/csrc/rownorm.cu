@@ -756,6 +756,8 @@ extern "C" int bgnn_rms_norm(bgnn_ctx* ctx, int x_type, const void* x, uint64_t 
   }
   BGNN_REQUIRE(ctx, x && weight && out, "rms_norm: NULL argument");
   BGNN_REQUIRE(ctx, !residual || total, "rms_norm: a residual needs a buffer for the sum");
+  BGNN_REQUIRE(ctx, !residual || total != residual || rows == 1 || ld_res == cols,
+               "rms_norm: the sum in the residual's buffer needs its row stride, the row length");
   BGNN_REQUIRE(ctx, out_type != BGNN_E4M3 || scale, "rms_norm: an e4m3 output needs scales");
   BGNN_REQUIRE(ctx, ld_x >= cols && (!residual || ld_res >= cols),
                "rms_norm: row stride below the row length");

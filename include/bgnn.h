@@ -561,7 +561,7 @@ BGNN_API int bgnn_link_scores(bgnn_ctx* ctx, const float* emb, uint32_t num_node
 /* Root-mean-square norm with the residual's addition:
  *   t = x + residual, rounded to the residual's type -> total [rows, cols]
  *       (t = x and total unused when residual is NULL; total may be the
- *       residual's own buffer when ld_res == cols)
+ *       residual's own buffer when ld_res == cols, which is checked)
  *   y = t * (mean(t^2) + eps)^(-1/2) * weight
  *   out = y, or for BGNN_E4M3 y / scale[row] with scale = max|y| / 448 (1 for
  *       an all-zero row, 0 without columns; e4m3 rounds to nearest even).
@@ -590,7 +590,8 @@ BGNN_API int bgnn_rms_norm_backward(bgnn_ctx* ctx, int grad_type, const void* gr
  * (x_scale [m], w_scale [n]; NULL otherwise).  bias [n], residual and out are
  * f32, bf16 or f16; bias and residual may be NULL.  act: bgnn_act, evaluated
  * in f32.  An operand whose rows do not start on 16 bytes is copied to rows
- * that do.  out may be the residual's own buffer. */
+ * that do.  out may be the residual's own buffer, with its type and row
+ * stride; another type or stride there is refused. */
 BGNN_API int bgnn_linear_fused(bgnn_ctx* ctx, int type, const void* x, uint64_t ld_x,
                                const float* x_scale, const void* w, uint64_t ld_w,
                                const float* w_scale, uint64_t m, uint32_t k, uint32_t n,
