@@ -51,11 +51,12 @@ constexpr float LN2 = 0.6931471805599453f;
 // An exponent on its way into 2^a and a 2^a: not below -150, where 2^a is 0, so
 // that a 2^a is never -inf * 0 (x - m may be -inf beside a mask of the type's
 // lowest value).  NaN stays NaN.
-__device__ __forceinline__ float floored(float a) {
+__device__ __forceinline__ float not_below(float a, float least) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(-150.0f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(least));
   return r;
 }
+__device__ __forceinline__ float floored(float a) { return not_below(a, -150.0f); }
 __device__ __forceinline__ float exponent(float d) { return floored(d * LOG2E); }
 
 struct Stat {
@@ -576,10 +577,12 @@ struct LogpBwdArgs {
 // such a row's m and log S are summed again by every block that works on it.
 constexpr float LSE_EXACT = 128.0f;
 
-// an element's gradient; x -inf: not left, and all of an empty row: none
+// an element's gradient; x -inf: not left, and all of an empty row: none.  log p
+// not below -104, where p is 0: gh times a log p near the type's lowest value is
+// infinite, and p times that NaN.
 __device__ __forceinline__ float grad_of(float x, float m, float ls, float k0, float gl, float gh,
                                          bool hit) {
-  const float lp = (x - m) - ls;
+  const float lp = not_below((x - m) - ls, -104.0f);
   const float d = ex2(lp * LOG2E) * fmaf(-gh, lp, k0);
   return x == -INFINITY ? 0.0f : hit ? d + gl : d;
 }
