@@ -23,7 +23,7 @@ import numpy as np
 
 from . import _lib
 from .backend import get_context, ptr
-from .blocks import logProbs
+from .blocks import TOP_MAX, logProbs
 from .graph import GraphData
 from .layers import GATConv, GCNConv, GINConv, Module, SAGEConv, _param, _torch, next_dropout_seed
 from .nn import ELU, Dropout, LeakyReLU, Linear, ReLU, Sequential, Sigmoid, Softmax
@@ -250,8 +250,9 @@ class LearningPathRecommender(Module):
         probability among the nodes not yet mastered, the entropy of that
         choice, and the topK alternatives (eval mode; no counterpart in the
         reference).  A mastered node has probability zero; equal scores come
-        in ascending node order, as in recommend."""
+        in ascending node order, as in recommend, and topK may be any."""
         torch = _torch()
+        topK = int(topK)
         if not 0 <= int(chosenNode) < graph.numNodes:
             raise ValueError(f"chosenNode {chosenNode} out of bounds for {graph.numNodes} nodes")
         self.eval()
@@ -260,7 +261,12 @@ class LearningPathRecommender(Module):
         m[[int(i) for i in masteredNodes]] = 1
         mask = torch.from_numpy(m).to(scores.device)
         target = torch.tensor([int(chosenNode)], dtype=torch.int32, device=scores.device)
-        logp, entropy, _, ids, top = logProbs(scores, target, mask=mask, topK=int(topK))
+        logp, entropy, _, ids, top = logProbs(scores, target, mask=mask, topK=min(topK, TOP_MAX))
+        if topK > TOP_MAX and graph.numNodes > TOP_MAX:  # longer than the kernel's list: sorted
+            left = scores.masked_fill(mask.bool() | scores.isnan(), -torch.inf)
+            v, ids = (t[:, :topK] for t in torch.sort(left, dim=1, descending=True, stable=True))
+            top = (v - v[:, :1]) + top[:, :1]  # x - max - log sum, as the kernel computes it
+            ids = ids.masked_fill(v == -torch.inf, -1)
         alternatives = []
         if topK:
             alternatives = [{"nodeIndex": i, "logProb": v, "rank": r + 1}
