@@ -278,10 +278,27 @@ class GatedFeedForward(Module):
         out = linearFused(h, self.p("down").to(half), residual=x, outType=torch.float32)
         return _wrap(input, out)
 
+    @staticmethod
+    def _into_f16(grad_out):
+        """(grad_out scaled by a power of two and in f16, the inverse): the
+        largest magnitude becomes 0.5 to 1, less where more than 4,096 rows add
+        up, so that neither a mean over many rows falls into f16's subnormals
+        nor a sum leaves its range."""
+        torch = _torch()
+        rows = grad_out.numel() // max(1, grad_out.shape[-1])
+        if grad_out.numel() == 0:
+            return grad_out.to(torch.float16), 1.0
+        top = -max(0, (rows - 1).bit_length() - 12)
+        by = (top - torch.frexp(grad_out.abs().amax())[1]).clamp(-126, 126)
+        one = torch.ones((), device=grad_out.device)
+        return (grad_out * torch.ldexp(one, by)).to(torch.float16), torch.ldexp(one, -by)
+
     def backward(self, input, grad_out) -> dict:
         """Gradients of forward(input) for grad_out [rows, features] (f32):
         {"x", "norm", "gate", "up", "down"}, f32.  The 16-bit activations are
-        computed once more from the input; nothing of the forward is kept."""
+        computed once more from the input; nothing of the forward is kept.
+        The gradients between the products, and those of gate, up and down, are
+        rounded to ``type`` once on their way; grad_out may be of any size."""
         if self.type == "e4m3":
             raise NotImplementedError("backward with e4m3 operands: train in bf16 or f16")
         x = _tensor_on_device(self, input)
@@ -289,8 +306,11 @@ class GatedFeedForward(Module):
         gate, up, down = (self.p(k).to(half) for k in ("gate", "up", "down"))
         n, _, _ = rmsNorm(x, self.p("norm"), eps=self.eps, outType=half)
         h = gatedLinear(n, gate, up, act=self.act)
-        gh, gdown, _ = linearFusedBackward(grad_out.to(half), h, down)
+        g, back = self._into_f16(grad_out) if self.type == "f16" else (grad_out.to(half), None)
+        gh, gdown, _ = linearFusedBackward(g, h, down)
         gn, ggate, gup, _, _ = gatedLinearBackward(gh, n, gate, up, act=self.act)
+        if back is not None:
+            gn, ggate, gup, gdown = (v.float() * back for v in (gn, ggate, gup, gdown))
         gx, gnorm = rmsNormBackward(gn, x, self.p("norm"), eps=self.eps, gradTotal=grad_out)
         return {"x": gx, "norm": gnorm, "gate": ggate.float(), "up": gup.float(),
                 "down": gdown.float()}
