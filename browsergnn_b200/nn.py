@@ -257,11 +257,13 @@ class GatedFeedForward(Module):
         return torch.float16 if self.type == "f16" else torch.bfloat16
 
     def _eight(self, name):
-        """A weight in e4m3 with one scale a row."""
+        """A weight in e4m3 with one scale a row, not below the smallest normal
+        number (as rmsNorm's): amax / 448 of a tiny row rounds to 0."""
         torch = _torch()
         w = self.p(name)
         amax = w.abs().amax(dim=1)
-        scale = torch.where(amax > 0, amax / 448.0, torch.ones_like(amax))
+        scale = torch.where(amax > 0, (amax / 448.0).clamp_min(torch.finfo(w.dtype).tiny),
+                            torch.ones_like(amax))
         return (w / scale[:, None]).to(torch.float8_e4m3fn), scale
 
     def forward(self, input):
