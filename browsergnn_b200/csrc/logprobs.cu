@@ -570,12 +570,22 @@ struct LogpBwdArgs {
   const float* g_ent;  // either may be NULL
   void* dx;            // [rows, cols]
   uint32_t splits, seg;
+  float2* far;         // [rows, far_splits] (m, S) of the far rows' segments, or NULL
+  uint32_t far_splits, far_seg;
   int* err;
 };
 
 // From |lse| = 128 on, its last bit is worth 2^-17 and more of a probability:
-// such a row's m and log S are summed again by every block that works on it.
+// such a row's m and log S are summed again, by every block that works on it or,
+// where a row has many blocks, by k_logp_far before them.
 constexpr float LSE_EXACT = 128.0f;
+__device__ __forceinline__ bool far_row(float lse) {
+  return fabsf(lse) >= LSE_EXACT && fabsf(lse) < INFINITY;
+}
+// Blocks of a row from which k_logp_far sums it: a far row of 100,000 f32 takes
+// 5.6 us with it and 18 without, one of 2.45M 11 and 595; the launch costs near
+// ones 1.2 us (2.0 -> 3.1, 4.8 -> 6.1).
+constexpr uint32_t FAR_SPLITS = 32;
 
 // an element's gradient; x -inf: not left, and all of an empty row: none.  log p
 // not below -104, where p is 0: gh times a log p near the type's lowest value is
@@ -605,7 +615,7 @@ __global__ void __launch_bounds__(256) k_logp_bwd_short(const LogpBwdArgs a) {
     auto at = [&](uint32_t e) {
       return mr && mr[e] ? -INFINITY : Elt<DT>::get(xr[e]);
     };
-    if (fabsf(ls) >= LSE_EXACT && fabsf(ls) < INFINITY) {
+    if (far_row(ls)) {
       Stat t = {-INFINITY, 0.0f, 0.0f};
       for (uint32_t e = lane; e < a.cols; e += 32) {
         const float x = at(e);
@@ -619,6 +629,43 @@ __global__ void __launch_bounds__(256) k_logp_bwd_short(const LogpBwdArgs a) {
     for (uint32_t e = lane; e < a.cols; e += 32)
       dr[e] = Elt<DT>::put(grad_of(at(e), m, ls, k0, gl, gh, e == c));
   }
+}
+
+// m and S over the block's threads, in every thread; `again`: a loop's next call
+// waits for the readers of the last
+__device__ __forceinline__ Stat block_sum(float (&sm_m)[8], float (&sm_s)[8], Stat t, bool again) {
+  t = warp_stat(t);
+  if (again) __syncthreads();
+  if ((threadIdx.x & 31) == 0) sm_m[threadIdx.x >> 5] = t.m, sm_s[threadIdx.x >> 5] = t.s;
+  __syncthreads();
+  t = {sm_m[0], sm_s[0], 0.0f};
+  for (int i = 1; i < 8; i++) t = stat_merge(t, {sm_m[i], sm_s[i], 0.0f});
+  return t;
+}
+
+// m and S of the far rows' segments: block = (row, segment)
+template <int DT>
+__global__ void __launch_bounds__(256) k_logp_far(const LogpBwdArgs a) {
+  __shared__ float sm_m[8], sm_s[8];
+  const uint64_t row = blockIdx.x / a.far_splits;
+  if (!far_row(a.lse[row])) return;
+  const uint32_t split = blockIdx.x % a.far_splits;
+  const elt_t<DT>* xr = static_cast<const elt_t<DT>*>(a.x) + row * a.ld;
+  const uint8_t* mr = a.mask ? a.mask + row * a.ld_mask : nullptr;
+  const int64_t lead = row_lead<DT>(xr);
+  const bool mask_vec = mr && (((uintptr_t)mr - (uintptr_t)lead) & 7u) == 0;
+  const int64_t first = (int64_t)split * a.far_seg - lead;
+  const int64_t lo = first > 0 ? first : 0;
+  const int64_t end = first + a.far_seg;
+  const int64_t hi = end < (int64_t)a.cols ? end : (int64_t)a.cols;
+  Stat t = {-INFINITY, 0.0f, 0.0f};
+  for (int64_t e = first + (int64_t)threadIdx.x * 8; e < hi; e += 256 * 8) {
+    float v[8];
+    load_left<DT>(xr, mr, mask_vec, e, lo, hi, v);
+    stat_add(t, v);
+  }
+  t = block_sum(sm_m, sm_s, t, false);
+  if (threadIdx.x == 0) a.far[blockIdx.x] = make_float2(t.m, t.s);
 }
 
 template <int DT>
@@ -647,19 +694,21 @@ __global__ void __launch_bounds__(256, 8) k_logp_bwd(const LogpBwdArgs a) {
       dev_raise(a.err, DEVERR_INDEX, c, 61);
     const float k0 = fmaf(-gh, h, -gl);
     float m = 0.0f, ls = lse;  // log p = (x - m) - ls
-    if (fabsf(lse) >= LSE_EXACT && fabsf(lse) < INFINITY) {
+    if (far_row(lse)) {
       Stat t = {-INFINITY, 0.0f, 0.0f};
-      for (int64_t e = (int64_t)threadIdx.x * 8 - lead; e < (int64_t)a.cols; e += 256 * 8) {
-        float v[8];
-        load_left<DT>(xr, mr, mask_vec, e, 0, a.cols, v);
-        stat_add(t, v);
+      if (a.far) {
+        for (uint32_t s = threadIdx.x; s < a.far_splits; s += 256) {
+          const float2 p = a.far[row * a.far_splits + s];
+          t = stat_merge(t, {p.x, p.y, 0.0f});
+        }
+      } else {
+        for (int64_t e = (int64_t)threadIdx.x * 8 - lead; e < (int64_t)a.cols; e += 256 * 8) {
+          float v[8];
+          load_left<DT>(xr, mr, mask_vec, e, 0, a.cols, v);
+          stat_add(t, v);
+        }
       }
-      t = warp_stat(t);
-      __syncthreads();  // the last unit's reads
-      if ((threadIdx.x & 31) == 0) sm_m[threadIdx.x >> 5] = t.m, sm_s[threadIdx.x >> 5] = t.s;
-      __syncthreads();
-      t = {sm_m[0], sm_s[0], 0.0f};
-      for (int i = 1; i < 8; i++) t = stat_merge(t, {sm_m[i], sm_s[i], 0.0f});
+      t = block_sum(sm_m, sm_s, t, true);
       m = t.m;
       ls = logf(t.s);
     }
@@ -738,6 +787,15 @@ int run_logp_bwd(bgnn_ctx* ctx, LogpBwdArgs a) {
     return BGNN_OK;
   }
   cut_rows(ctx, a.rows, a.cols, 8, 2048, &a.splits, &a.seg);
+  DevTmp far;
+  if (a.splits >= FAR_SPLITS) {
+    cut_rows(ctx, a.rows, a.cols, 2, 4096, &a.far_splits, &a.far_seg);
+    const uint64_t parts = (uint64_t)a.rows * a.far_splits;  // at most two blocks an SM
+    BGNN_TRY(bgnn_tmp_alloc(ctx, far, parts * sizeof(float2)));
+    a.far = far.as<float2>();
+    k_logp_far<DT><<<(unsigned)parts, 256, 0, ctx->stream>>>(a);
+    BGNN_LAUNCHED(ctx);
+  }
   const uint64_t units = (uint64_t)a.rows * a.splits, cap = (uint64_t)ctx->num_sms * 64;
   k_logp_bwd<DT><<<(unsigned)(units < cap ? units : cap), 256, 0, ctx->stream>>>(a);
   BGNN_LAUNCHED(ctx);
