@@ -42,7 +42,8 @@ class CudaContext:
             raise RuntimeError("the cuda backend needs a CUDA device (there is no CPU fallback)")
         self.lib = _lib.load()
         h = ctypes.c_void_p()
-        _lib.check(self.lib.bgnn_ctx_create(int(device), ctypes.byref(h)))
+        with torch.cuda.device(int(device)):  # creating sets the device; the caller's comes back
+            _lib.check(self.lib.bgnn_ctx_create(int(device), ctypes.byref(h)))
         self.h = h
         self.device = int(device)
         self._stream = None

@@ -47,9 +47,40 @@ def ctx(monkeypatch):
     lib.bgnn_ctx_create = lambda device, out: 0
     monkeypatch.setattr(_lib, "load", lambda: lib)
     monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "device", Device)
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: STREAM.s,
                         raising=False)
     return backend.CudaContext(0)
+
+
+class Device:
+    """torch.cuda.device over a fake current device."""
+
+    current = 0
+
+    def __init__(self, index):
+        self.index = index
+
+    def __enter__(self):
+        self.before, Device.current = Device.current, self.index
+
+    def __exit__(self, *exc):
+        Device.current = self.before
+
+
+def test_a_new_context_leaves_the_current_device(ctx, monkeypatch):
+    """A first call with tensors of another device than the current one."""
+    made = []
+
+    def create(device, out):
+        made.append(device)
+        Device.current = device  # as cudaSetDevice in the library does
+        return 0
+
+    monkeypatch.setattr(ctx.lib, "bgnn_ctx_create", create)
+    monkeypatch.setattr(Device, "current", 0)
+    assert backend.CudaContext(1).device == 1
+    assert made == [1] and Device.current == 0
 
 
 @pytest.mark.parametrize("how", ["call", "call_on", "synchronize"])
