@@ -42,7 +42,7 @@ class CudaContext:
             raise RuntimeError("the cuda backend needs a CUDA device (there is no CPU fallback)")
         self.lib = _lib.load()
         h = ctypes.c_void_p()
-        with torch.cuda.device(int(device)):  # creating sets the device; the caller's comes back
+        with torch.cuda.device(torch.cuda.current_device()):  # creating sets the device
             _lib.check(self.lib.bgnn_ctx_create(int(device), ctypes.byref(h)))
         self.h = h
         self.device = int(device)

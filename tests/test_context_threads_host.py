@@ -48,6 +48,7 @@ def ctx(monkeypatch):
     monkeypatch.setattr(_lib, "load", lambda: lib)
     monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
     monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: Device.current)
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: STREAM.s,
                         raising=False)
     return backend.CudaContext(0)
@@ -81,6 +82,11 @@ def test_a_new_context_leaves_the_current_device(ctx, monkeypatch):
     monkeypatch.setattr(Device, "current", 0)
     assert backend.CudaContext(1).device == 1
     assert made == [1] and Device.current == 0
+    monkeypatch.setattr(ctx.lib, "bgnn_ctx_create", lambda device, out: 3)  # no such device
+    monkeypatch.setattr(_lib, "check", lambda rc, h=None: (_ for _ in ()).throw(RuntimeError(rc)))
+    with pytest.raises(RuntimeError, match="3"):
+        backend.CudaContext(99)
+    assert Device.current == 0
 
 
 @pytest.mark.parametrize("how", ["call", "call_on", "synchronize"])
