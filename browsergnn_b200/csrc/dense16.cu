@@ -75,14 +75,25 @@ enum Epi : int {
   EPI_LINEAR,
   EPI_LINEAR_F32,
   EPI_GATED,
+  EPI_GATED_F32,
   EPI_LINEAR_BWD,
   EPI_GATED_BWD,
   EPI_PARTIAL
 };
-// k blocks whose products one accumulator takes before they are added in f32
-// registers, where the result stays f32 (EPI_LINEAR_F32)
+// the B tile holds two weights
+template <int EPI>
+constexpr bool TWO_WEIGHTS = EPI == EPI_GATED || EPI == EPI_GATED_F32 || EPI == EPI_GATED_BWD;
+// The result stays f32: an accumulator takes the products of PIECE k blocks, and
+// these pieces are added in f32 registers.  (The tensor cores cut their additions,
+// of 16 products each, short by up to 2^-23 of the sum so far: 8,192 positive
+// terms lose 3e-5 in one accumulator and 4e-7 in pieces.  Gated 16,384 x 4,096 ->
+// 4,096 takes 836 us in pieces, 769 without.)
+template <int EPI>
+constexpr bool PIECES = EPI == EPI_LINEAR_F32 || EPI == EPI_GATED_F32;
 constexpr uint32_t PIECE = 8;
-constexpr uint32_t MAX_PER = 512;  // k blocks of a dw range
+// k blocks of a dw range: 32,768 products, whose additions lose at most 2.4e-4 of
+// their sum, half of what the result's rounding to f16 may
+constexpr uint32_t MAX_PER = 512;
 
 // a, b: the operands of each contraction segment (dx), of each batch (dw: a), or
 // the two weights of a gated product (b).
@@ -450,7 +461,7 @@ struct Tiles {
 template <int EPI, int CG>
 __global__ void __launch_bounds__(THREADS, 1)
     k_dense16(const __grid_constant__ Maps maps, const GemmArgs g) {
-  constexpr bool TWO = EPI == EPI_GATED || EPI == EPI_GATED_BWD;  // B tile of two weights
+  constexpr bool TWO = TWO_WEIGHTS<EPI>;  // B tile of two weights
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = s_addr(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;  // swizzle atoms start on 1024 bytes
@@ -579,7 +590,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             const uint32_t last = kb_last(ti);
             uint32_t kb = kb_first(ti);
             do {  // a piece of the contraction into one accumulator
-              const uint32_t e = EPI == EPI_LINEAR_F32 && last - kb > PIECE ? kb + PIECE : last;
+              const uint32_t e = PIECES<EPI> && last - kb > PIECE ? kb + PIECE : last;
               if (!mbar_wait(b_acce + 8 * buf, aph ^ 1u, abort_flag, g.err, 71)) return false;
               tc_fence_after();
               const uint32_t d = tmem + buf * bn;
@@ -781,8 +792,25 @@ __global__ void __launch_bounds__(THREADS, 1)
       };
 
       if (group * 32 < wn) ask(ti.n0 + group * 32);
-      if constexpr (EPI == EPI_LINEAR_F32) {
-        // pieces of the contraction added in f32 registers, rounded to nearest
+      auto gated_out = [&](float (&v)[32], float (&u)[32], uint32_t col0) {
+        scaled(v, col0, 0);
+        scaled(u, col0, 1);
+        with_act(g.act, [&](auto act) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float2 f = mul2(act_two<decltype(act)::value>(make_float2(v[j], v[j + 1]), g.act_p),
+                                  make_float2(u[j], u[j + 1]));
+            v[j] = f.x;
+            v[j + 1] = f.y;
+          }
+        });
+        give(v, col0, g.out[0], g.ld_out, g.out_type);
+      };
+      if constexpr (PIECES<EPI>) {
+        // pieces of the contraction added in f32 registers, rounded to nearest:
+        // this warp's two chunks of columns, or both products of its one chunk
+        const uint32_t step = TWO ? wn : 128u;
+        auto mine = [&](int i) { return TWO ? group * 32 < wn : group * 32 + i * 128 < wn; };
         float sum[2][32];
 #pragma unroll
         for (int i = 0; i < 2; i++)
@@ -798,10 +826,9 @@ __global__ void __launch_bounds__(THREADS, 1)
           const uint32_t acc = tmem + lanes + buf * g.bn;
 #pragma unroll
           for (int i = 0; i < 2; i++) {
-            const uint32_t c = group * 32 + i * 128;
-            if (c < wn && any_k) {
+            if (mine(i) && any_k) {
               float v[32];
-              tmem_ld32(acc + c, v);
+              tmem_ld32(acc + group * 32 + i * step, v);
               tmem_wait_ld(v);
 #pragma unroll
               for (int j = 0; j < 32; j++) sum[i][j] += v[j];
@@ -811,12 +838,17 @@ __global__ void __launch_bounds__(THREADS, 1)
           kb += PIECE;
         } while (kb < k_last);
         if (gave_up) break;
+        if constexpr (TWO) {
+          const uint32_t c = group * 32;
+          if (c < wn && ti.n0 + c < g.n) gated_out(sum[0], sum[1], ti.n0 + c);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-          const uint32_t c = group * 32 + i * 128;
-          if (c < wn && ti.n0 + c < g.n) {
-            if (i) ask(ti.n0 + c);
-            linear_out(sum[i], ti.n0 + c);
+          for (int i = 0; i < 2; i++) {
+            const uint32_t c = group * 32 + i * 128;
+            if (c < wn && ti.n0 + c < g.n) {
+              if (i) ask(ti.n0 + c);
+              linear_out(sum[i], ti.n0 + c);
+            }
           }
         }
       } else {
@@ -867,19 +899,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             give(v, col0, g.out[0], g.ld_out, g.out_type);
             bias_sums(v, col0, g.bsum[0]);
           } else if constexpr (EPI == EPI_GATED) {
-            scaled(v, col0, 0);
-            scaled(u, col0, 1);
-            with_act(g.act, [&](auto act) {
-#pragma unroll
-              for (int j = 0; j < 32; j += 2) {
-                const float2 f =
-                    mul2(act_two<decltype(act)::value>(make_float2(v[j], v[j + 1]), g.act_p),
-                         make_float2(u[j], u[j + 1]));
-                v[j] = f.x;
-                v[j + 1] = f.y;
-              }
-            });
-            give(v, col0, g.out[0], g.ld_out, g.out_type);
+            gated_out(v, u, col0);
           } else {
             scaled(v, col0, 0);
             scaled(u, col0, 1);
@@ -1189,7 +1209,7 @@ int launch_cg(bgnn_ctx* ctx, const Maps& maps, const GemmArgs& g, uint64_t tiles
 
 template <int EPI>
 int launch(bgnn_ctx* ctx, const Maps& maps, GemmArgs& g, const Shape& s) {
-  constexpr bool TWO = EPI == EPI_GATED || EPI == EPI_GATED_BWD;
+  constexpr bool TWO = TWO_WEIGHTS<EPI>;
   g.idesc = make_idesc(g.in_type, g.a_mn, g.b_mn, s);
   g.fp8 = g.in_type == BGNN_E4M3;
   g.err = ctx->d_err;
@@ -1203,7 +1223,7 @@ int launch(bgnn_ctx* ctx, const Maps& maps, GemmArgs& g, const Shape& s) {
 // z = x w^T (one weight or two) with the epilogue of `EPI`
 template <int EPI>
 int run_nt(bgnn_ctx* ctx, GemmArgs& g, Mat x, const Mat (&w)[2], uint32_t k) {
-  constexpr bool TWO = EPI == EPI_GATED || EPI == EPI_GATED_BWD;
+  constexpr bool TWO = TWO_WEIGHTS<EPI>;
   if constexpr (EPI == EPI_LINEAR || EPI == EPI_GATED)
     if (few_rows(g.m, k, g.n, TWO)) {
       RowsArgs r = {};
@@ -1236,8 +1256,9 @@ int run_nt(bgnn_ctx* ctx, GemmArgs& g, Mat x, const Mat (&w)[2], uint32_t k) {
   g.a_mn = g.b_mn = 0;
   g.nkb[0] = blocks_of(k, g.in_type == BGNN_E4M3 ? 128 : 64);
   g.nkb[1] = 0;
+  const bool f32_out = g.out_type == BGNN_F32;  // the pieces' registers hold 256 columns
   const Shape sh = pick_shape(ctx, g.m, g.n, 1, TWO, TWO ? 64 : 32, g.nkb[0],
-                              EPI != EPI_LINEAR || g.out_type != BGNN_F32);
+                              EPI == EPI_LINEAR_BWD || EPI == EPI_GATED_BWD || !f32_out);
   set_tile(&g, sh);
   if (k) {
     BGNN_TRY(tma_ready(ctx, g.in_type, &x, tx));
@@ -1255,7 +1276,9 @@ int run_nt(bgnn_ctx* ctx, GemmArgs& g, Mat x, const Mat (&w)[2], uint32_t k) {
     BGNN_TRY(make_chunk_map(ctx, &maps.in, g.other_type, in));
   }
   if constexpr (EPI == EPI_LINEAR)
-    if (g.out_type == BGNN_F32) return launch<EPI_LINEAR_F32>(ctx, maps, g, sh);
+    if (f32_out) return launch<EPI_LINEAR_F32>(ctx, maps, g, sh);
+  if constexpr (EPI == EPI_GATED)
+    if (f32_out && g.nkb[0] > PIECE) return launch<EPI_GATED_F32>(ctx, maps, g, sh);
   return launch<EPI>(ctx, maps, g, sh);
 }
 
@@ -1307,7 +1330,7 @@ int run_dw(bgnn_ctx* ctx, int type, uint32_t m, uint32_t n, uint32_t k, const Ma
   }
   set_tile(&g, sh);
   // ranges so that every SM has a tile, each of at least 8 k blocks, and of at
-  // most MAX_PER: the tensor cores' own additions cost about 2^-24 a block
+  // most MAX_PER
   const uint64_t tiles = (uint64_t)blocks_of(n, BM * sh.cg) * blocks_of(k, g.bn) * terms;
   uint64_t s = tiles * sh.cg >= (uint64_t)ctx->num_sms ? 1 : ctx->num_sms / (tiles * sh.cg);
   if (s > (g.nkb[0] + 7) / 8) s = (g.nkb[0] + 7) / 8;
