@@ -659,9 +659,10 @@ unsigned row_grid(const bgnn_ctx* ctx, uint64_t rows, const RowShape& r) {
   return (unsigned)(want < cap ? want : cap);
 }
 
+constexpr uint32_t STATIC_SHARED = 64 * sizeof(float2);  // the kernels' `red`
 template <class K, class... A>
 int launch_rows(bgnn_ctx* ctx, K kernel, unsigned grid, const RowShape& r, A... args) {
-  if (r.shared > 48 * 1024)
+  if (r.shared + STATIC_SHARED > 48 * 1024)  // what a launch may take without being asked for
     BGNN_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         (int)r.shared));
   kernel<<<grid, r.block, r.shared, ctx->stream>>>(args...);

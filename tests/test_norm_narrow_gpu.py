@@ -81,3 +81,23 @@ def test_modules_of_one_to_four_features():
         out, grads = m.forward(x), m.backward(x, x)
         assert out.shape == x.shape and torch.isfinite(out).all()
         assert all(torch.isfinite(v).all() for v in grads.values())
+
+
+@pytest.mark.parametrize("t", [BF, F16])
+@pytest.mark.parametrize("cols", [1004, 1005, 1012, 1016, 1019, 1020, 1021, 1024])
+def test_backward_at_the_shared_memory_of_a_launch(cols, t):
+    """A block's column sums, its staged rows and its static shared memory come
+    to 48 KB, the most that a launch has without asking, at about 1,020 columns."""
+    g = gen(cols)
+    w = normal(g, cols)
+    T0, G0 = normal(g, 40, cols, t=t), normal(g, 40, cols, t=t)
+    T, G, W = T0.double(), G0.double(), w.double()
+    s = (T.pow(2).mean(1, keepdim=True) + 1e-6).rsqrt()
+    xh = T * s
+    for how in ("plain", "odd"):
+        gx, gw = bg.rmsNormBackward(wide(G0, how), wide(T0, how), w)
+        c = (G * W * xh).mean(1, keepdim=True)
+        mag = s * ((G * W).abs() + xh.abs() * (G * W * xh).abs().mean(1, keepdim=True))
+        want = s * (G * W - xh * c)
+        within(gx, want, U[t] * want.abs() + (2 * cols + 32) * 2.0 ** -24 * mag + TINY[t], how)
+        within(gw, (G * xh).sum(0), (40 + cols + 32) * 2.0 ** -24 * (G * xh).abs().sum(0), how)
