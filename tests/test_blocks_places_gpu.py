@@ -172,3 +172,26 @@ def test_modules_in_a_sequential():
     for part in m._modules.values():
         y = part.forward(y)
     assert torch.equal(m.forward(x), y)
+
+
+@pytest.mark.parametrize("type", ["bf16", "f16", "e4m3"])
+def test_modules_captured(type):
+    """Forward and gradients recorded once and replayed on other features."""
+    g = gen(6)
+    x, other, go = (normal(g, 300, 24) for _ in range(3))
+    m = bg.Sequential([bg.RMSNorm(features=24),
+                       bg.GatedFeedForward(features=24, hiddenFeatures=72, type=type)])
+    ffn = m._modules["1"]
+
+    def run():
+        out = [m.forward(x)]
+        if type != "e4m3":
+            out += [v for _, v in sorted(ffn.backward(x, go).items())]
+        return out
+
+    calls = bg.CapturedForward(run)
+    x.copy_(other)
+    go.mul_(1e-6)
+    got = [v.clone() for v in calls()]
+    assert all(torch.equal(a, b) for a, b in zip(got, run()))
+    calls.close()
