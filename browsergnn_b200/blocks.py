@@ -15,8 +15,9 @@ The reference has no counterpart: its Linear (src/nn/linear.ts) and softmax
 (src/core/tensor.ts:435-499) are f32 and stay `Linear`, `Softmax` and
 `LogSoftmax`.  Tensors are CUDA tensors of one device, one- or two-dimensional
 ([features] is one row), rows any distance apart; results are fresh tensors on
-torch's current stream.  Gradients are explicit calls, as the layers'
-``backward`` is.  Errors in arguments raise ValueError or TypeError, what the
+torch's current stream.  Host threads may call at once, each on its own
+stream.  Gradients are explicit calls, as the layers' ``backward`` is.  Errors
+in arguments raise ValueError or TypeError, what the
 library reports raises BGNNError.
 """
 from __future__ import annotations
@@ -157,7 +158,8 @@ def rmsNorm(x, weight, residual=None, eps: float = 1e-6, outType=None):
     x is f32, bf16 or f16, residual x's type or f32.  outType (x's type when
     None) f32, bf16, f16, or torch.float8_e4m3fn: then ``out * scale[row]`` is
     the result, scale [rows] f32 being the row's largest magnitude / 448;
-    scale is None for the other types."""
+    scale is None for the other types.  The squares are added in f32: rows
+    whose sum of squares passes 3.4e38 give 0."""
     torch = _torch()
     t, one = _rows(x, "x")
     rows, cols = t.shape

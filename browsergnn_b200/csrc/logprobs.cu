@@ -16,9 +16,10 @@
 // does, which are read once more (from L2) and ranked by counting: 157 us for
 // 8,192 x 32,000 bf16, k = 20 (3.3 TB/s), 117 us without a list.  (Keeping the
 // list sorted in a warp's lanes while reading took 565 us; it is what a row with
-// hundreds of equal logits at the border falls back to.)  A long row is split over blocks
-// and joined by k_logp_join; short rows take a warp each.  The logits (and masks) are read once; about seven
-// instructions an element, one of them 2^x, bound it before memory does.
+// hundreds of equal logits at the border falls back to.)  A long row is split
+// over blocks and joined by k_logp_join; short rows take a warp each.  The logits
+// (and masks) are read once; about seven instructions an element, one of them
+// 2^x, bound it before memory does.
 #include "lowp.cuh"
 
 namespace {

@@ -565,6 +565,8 @@ BGNN_API int bgnn_link_scores(bgnn_ctx* ctx, const float* emb, uint32_t num_node
  *   y = t * (mean(t^2) + eps)^(-1/2) * weight
  *   out = y, or for BGNN_E4M3 y / scale[row] with scale = max|y| / 448 (1 for
  *       an all-zero row, 0 without columns; e4m3 rounds to nearest even).
+ * The squares are added in f32: a row whose sum of squares passes 3.4e38 gives
+ * 0, one of zeros with eps == 0 NaN.
  * x f32, bf16 or f16; the residual has x's type or f32; weight [cols] any of
  * the three; out f32, bf16, f16 or e4m3 (scale [rows], else NULL).  A row that
  * holds a NaN or an infinity gives NaN in what it touches, and a NaN scale or
@@ -591,7 +593,11 @@ BGNN_API int bgnn_rms_norm_backward(bgnn_ctx* ctx, int grad_type, const void* gr
  * f32, bf16 or f16; bias and residual may be NULL.  act: bgnn_act, evaluated
  * in f32.  An operand whose rows do not start on 16 bytes is copied to rows
  * that do.  out may be the residual's own buffer, with its type and row
- * stride; another type or stride there is refused. */
+ * stride; another type or stride there is refused.  The tensor cores cut each
+ * addition of 16 products (e4m3: 32) short by up to 2^-23 of the sum so far;
+ * results in f32 are summed in pieces of 512 (1,024) products rounded to
+ * nearest, results in 16 bits in one sum, whose loss stays below their rounding
+ * up to k = 65,536 (f16). */
 BGNN_API int bgnn_linear_fused(bgnn_ctx* ctx, int type, const void* x, uint64_t ld_x,
                                const float* x_scale, const void* w, uint64_t ld_w,
                                const float* w_scale, uint64_t m, uint32_t k, uint32_t n,
