@@ -613,14 +613,22 @@ __device__ __forceinline__ bool far_row(float lse) {
 // ones 1.2 us (2.0 -> 3.1, 4.8 -> 6.1).
 constexpr uint32_t FAR_SPLITS = 32;
 
-// an element's gradient; x -inf: not left, and all of an empty row: none.  log p
+// two elements' gradients; x -inf: not left, and all of an empty row: none.  log p
 // not below -104, where p is 0: gh times a log p near the type's lowest value is
 // infinite, and p times that NaN.
+__device__ __forceinline__ float2 grad_two(float2 x, float m, float ls, float k0, float gl, float gh,
+                                           bool hit0, bool hit1) {
+  const float2 d = add2(add2(x, make_float2(-m, -m)), make_float2(-ls, -ls));
+  const float2 lp = make_float2(not_below(d.x, -104.0f), not_below(d.y, -104.0f));
+  const float2 t = mul2(lp, make_float2(LOG2E, LOG2E));
+  const float2 g = mul2(make_float2(ex2(t.x), ex2(t.y)),
+                        fma2(make_float2(-gh, -gh), lp, make_float2(k0, k0)));
+  return make_float2(x.x == -INFINITY ? 0.0f : hit0 ? g.x + gl : g.x,
+                     x.y == -INFINITY ? 0.0f : hit1 ? g.y + gl : g.y);
+}
 __device__ __forceinline__ float grad_of(float x, float m, float ls, float k0, float gl, float gh,
                                          bool hit) {
-  const float lp = not_below((x - m) - ls, -104.0f);
-  const float d = ex2(lp * LOG2E) * fmaf(-gh, lp, k0);
-  return x == -INFINITY ? 0.0f : hit ? d + gl : d;
+  return grad_two(make_float2(x, -INFINITY), m, ls, k0, gl, gh, hit, false).x;
 }
 
 // short rows: a warp a row, an element a lane at a time
@@ -742,8 +750,12 @@ __global__ void __launch_bounds__(256, 8) k_logp_bwd(const LogpBwdArgs a) {
       float v[8];
       load_left<DT>(xr, mr, mask_vec, e, lo, hi, v);
 #pragma unroll
-      for (int j = 0; j < 8; j++)
-        v[j] = grad_of(v[j], m, ls, k0, gl, gh, e + j == (int64_t)c);
+      for (int j = 0; j < 8; j += 2) {
+        const float2 d = grad_two(make_float2(v[j], v[j + 1]), m, ls, k0, gl, gh,
+                                  e + j == (int64_t)c, e + j + 1 == (int64_t)c);
+        v[j] = d.x;
+        v[j + 1] = d.y;
+      }
       if (out_vec && e >= lo && e + 8 <= hi) {
         store8<DT>(dr + e, v);
       } else {
