@@ -20,6 +20,8 @@
 // over blocks and joined by k_logp_join; short rows take a warp each.  The logits
 // (and masks) are read once; about seven instructions an element, one of them
 // 2^x, bound it before memory does.
+#include <atomic>
+
 #include "lowp.cuh"
 
 namespace {
@@ -596,22 +598,45 @@ struct LogpBwdArgs {
   const float* g_ent;  // either may be NULL
   void* dx;            // [rows, cols]
   uint32_t splits, seg;
-  float2* far;         // [rows, far_splits] (m, S) of the far rows' segments, or NULL
-  uint32_t far_splits, far_seg;
   int* err;
 };
 
 // From |lse| = 128 on, its last bit is worth 2^-17 and more of a probability:
-// such a row's m and log S are summed again, by every block that works on it or,
-// where a row has many blocks, by k_logp_far before them.
+// such a row is summed again.
 constexpr float LSE_EXACT = 128.0f;
 __device__ __forceinline__ bool far_row(float lse) {
   return fabsf(lse) >= LSE_EXACT && fabsf(lse) < INFINITY;
 }
-// Blocks of a row from which k_logp_far sums it: a far row of 100,000 f32 takes
-// 5.6 us with it and 18 without, one of 2.45M 11 and 595; the launch costs near
-// ones 1.2 us (2.0 -> 3.1, 4.8 -> 6.1).
-constexpr uint32_t FAR_SPLITS = 32;
+// Every block of a far row needs the sum, and a launch that makes it before costs
+// every call 5 to 7 us of the host's time.  So each block sums the row, and where
+// a row has many blocks, clusters of this many share that work: 1 x 2.45M f32
+// 45 us (each block alone 595), a near row 5.5 (4.8 without clusters; eight
+// blocks: 80 and 5.3).
+constexpr uint32_t FAR_CLUSTER = 16;
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+// *p of the cluster's block `rank`
+__device__ __forceinline__ float cluster_load(const float* p, uint32_t rank) {
+  uint32_t a;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+               : "=r"(a)
+               : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
 
 // two elements' gradients; x -inf: not left, and all of an empty row: none.  log p
 // not below -104, where p is 0: gh times a log p near the type's lowest value is
@@ -665,46 +690,45 @@ __global__ void __launch_bounds__(256) k_logp_bwd_short(const LogpBwdArgs a) {
   }
 }
 
-// m and S over the block's threads, in every thread; `again`: a loop's next call
-// waits for the readers of the last
-__device__ __forceinline__ Stat block_sum(float (&sm_m)[8], float (&sm_s)[8], Stat t, bool again) {
-  t = warp_stat(t);
-  if (again) __syncthreads();
-  if ((threadIdx.x & 31) == 0) sm_m[threadIdx.x >> 5] = t.m, sm_s[threadIdx.x >> 5] = t.s;
-  __syncthreads();
-  t = {sm_m[0], sm_s[0], 0.0f};
-  for (int i = 1; i < 8; i++) t = stat_merge(t, {sm_m[i], sm_s[i], 0.0f});
-  return t;
-}
-
-// m and S of the far rows' segments: block = (row, segment)
+// sum exp(x - lse) over a far row, in every thread of every block of the cluster
+// (or of the block, launched without one): the blocks take its vectors in turn,
+// and their sums are added in the order of their ranks.
 template <int DT>
-__global__ void __launch_bounds__(256) k_logp_far(const LogpBwdArgs a) {
-  __shared__ float sm_m[8], sm_s[8];
-  const uint64_t row = blockIdx.x / a.far_splits;
-  if (!far_row(a.lse[row])) return;
-  const uint32_t split = blockIdx.x % a.far_splits;
-  const elt_t<DT>* xr = static_cast<const elt_t<DT>*>(a.x) + row * a.ld;
-  const uint8_t* mr = a.mask ? a.mask + row * a.ld_mask : nullptr;
-  const int64_t lead = row_lead<DT>(xr);
-  const bool mask_vec = mr && (((uintptr_t)mr - (uintptr_t)lead) & 7u) == 0;
-  const int64_t first = (int64_t)split * a.far_seg - lead;
-  const int64_t lo = first > 0 ? first : 0;
-  const int64_t end = first + a.far_seg;
-  const int64_t hi = end < (int64_t)a.cols ? end : (int64_t)a.cols;
-  Stat t = {-INFINITY, 0.0f, 0.0f};
-  for (int64_t e = first + (int64_t)threadIdx.x * 8; e < hi; e += 256 * 8) {
+__device__ __forceinline__ float far_sum(const elt_t<DT>* xr, const uint8_t* mr, bool mask_vec,
+                                         int64_t lead, int64_t cols, float lse, float (&sm)[9]) {
+  const uint32_t rank = cluster_rank(), size = cluster_size();
+  float2 s = make_float2(0.0f, 0.0f);
+  const float2 minus = make_float2(-lse, -lse), log2e = make_float2(LOG2E, LOG2E);
+  for (int64_t e = (int64_t)(rank * 256 + threadIdx.x) * 8 - lead; e < cols; e += size * 256 * 8) {
     float v[8];
-    load_left<DT>(xr, mr, mask_vec, e, lo, hi, v);
-    stat_add(t, v);
+    load_left<DT>(xr, mr, mask_vec, e, 0, cols, v);
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      const float2 t = mul2(add2(make_float2(v[j], v[j + 1]), minus), log2e);
+      s = add2(s, make_float2(ex2(t.x), ex2(t.y)));
+    }
   }
-  t = block_sum(sm_m, sm_s, t, false);
-  if (threadIdx.x == 0) a.far[blockIdx.x] = make_float2(t.m, t.s);
+  float t = s.x + s.y;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  __syncthreads();  // the last far row's readers
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = t;
+  __syncthreads();
+  t = sm[0];
+  for (int i = 1; i < 8; i++) t += sm[i];
+  if (size > 1) {  // far rows are the same for all blocks of a cluster
+    if (threadIdx.x == 0) sm[8] = t;
+    cluster_sync();
+    t = 0.0f;
+    for (uint32_t i = 0; i < size; i++) t += cluster_load(&sm[8], i);
+    cluster_sync();  // no block goes on to write sm, or leaves, before all have read
+  }
+  return t;
 }
 
 template <int DT>
 __global__ void __launch_bounds__(256, 8) k_logp_bwd(const LogpBwdArgs a) {
-  __shared__ float sm_m[8], sm_s[8];
+  __shared__ float sm[9];
   const uint64_t units = (uint64_t)a.rows * a.splits;
   for (uint64_t u = blockIdx.x; u < units; u += gridDim.x) {
     const uint64_t row = u / a.splits;
@@ -728,23 +752,9 @@ __global__ void __launch_bounds__(256, 8) k_logp_bwd(const LogpBwdArgs a) {
       dev_raise(a.err, DEVERR_INDEX, c, 61);
     const float k0 = fmaf(-gh, h, -gl);
     float m = 0.0f, ls = lse;  // log p = (x - m) - ls
-    if (far_row(lse)) {
-      Stat t = {-INFINITY, 0.0f, 0.0f};
-      if (a.far) {
-        for (uint32_t s = threadIdx.x; s < a.far_splits; s += 256) {
-          const float2 p = a.far[row * a.far_splits + s];
-          t = stat_merge(t, {p.x, p.y, 0.0f});
-        }
-      } else {
-        for (int64_t e = (int64_t)threadIdx.x * 8 - lead; e < (int64_t)a.cols; e += 256 * 8) {
-          float v[8];
-          load_left<DT>(xr, mr, mask_vec, e, 0, a.cols, v);
-          stat_add(t, v);
-        }
-      }
-      t = block_sum(sm_m, sm_s, t, true);
-      m = t.m;
-      ls = logf(t.s);
+    if (far_row(lse)) {  // log p = (x - lse) - log sum exp(x - lse)
+      m = lse;
+      ls = logf(far_sum<DT>(xr, mr, mask_vec, lead, a.cols, lse, sm));
     }
     for (int64_t e = first + (int64_t)threadIdx.x * 8; e < hi; e += 256 * 8) {
       float v[8];
@@ -825,17 +835,30 @@ int run_logp_bwd(bgnn_ctx* ctx, LogpBwdArgs a) {
     return BGNN_OK;
   }
   cut_rows(ctx, a.rows, a.cols, 8, 2048, &a.splits, &a.seg);
-  DevTmp far;
-  if (a.splits >= FAR_SPLITS) {
-    cut_rows(ctx, a.rows, a.cols, 2, 4096, &a.far_splits, &a.far_seg);
-    const uint64_t parts = (uint64_t)a.rows * a.far_splits;  // at most two blocks an SM
-    BGNN_TRY(bgnn_tmp_alloc(ctx, far, parts * sizeof(float2)));
-    a.far = far.as<float2>();
-    k_logp_far<DT><<<(unsigned)parts, 256, 0, ctx->stream>>>(a);
-    BGNN_LAUNCHED(ctx);
-  }
+  const bool clusters = a.splits >= FAR_CLUSTER;
+  if (clusters)  // a cluster's blocks work on one row: whole clusters of them (some with nothing)
+    a.splits = (a.splits + FAR_CLUSTER - 1) / FAR_CLUSTER * FAR_CLUSTER;
   const uint64_t units = (uint64_t)a.rows * a.splits, cap = (uint64_t)ctx->num_sms * 64;
-  k_logp_bwd<DT><<<(unsigned)(units < cap ? units : cap), 256, 0, ctx->stream>>>(a);
+  if (clusters) {
+    static std::atomic<uint64_t> ready{0};  // devices (below 64) where 16 blocks are allowed
+    const uint64_t bit = ctx->device < 64 ? 1ull << ctx->device : 0;
+    if (!(ready.load(std::memory_order_relaxed) & bit)) {
+      BGNN_CUDA(ctx, cudaFuncSetAttribute(k_logp_bwd<DT>,
+                                          cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+      ready.fetch_or(bit, std::memory_order_relaxed);
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(units < cap ? units : cap));
+  cfg.blockDim = dim3(256);
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = FAR_CLUSTER;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = clusters ? 1 : 0;
+  BGNN_CUDA(ctx, cudaLaunchKernelEx(&cfg, k_logp_bwd<DT>, a));
   BGNN_LAUNCHED(ctx);
   return BGNN_OK;
 }
