@@ -1,5 +1,5 @@
-"""The choice head's gradient for long rows whose log-sum-exp is large: their
-sum is made once a row, not once a block."""
+"""The choice head's gradient for long rows whose log-sum-exp is large: such a
+row is summed again, by blocks that share the work."""
 import pytest
 import torch
 
@@ -38,7 +38,7 @@ def test_near_and_far_rows_together(rows, cols, t, masked):
     want = p * (-1 - E * (safe + H))
     want[:, 0] += some[:, 0].double()
     # near rows: half the last bit of lse (below 128, 2^-18) is an error of p; far
-    # ones: m and S in f32.  2^-15 of the terms covers either, and the entropy's.
+    # ones: x - lse and its exponentials' sum in f32.  2^-15 of the terms covers either, and the entropy's.
     mag = p * (1 + E.abs() * (safe.abs() + H + 1))
     tol = U[t] * want.abs() + 2.0 ** -15 * mag + 2.0 ** -23 + TINY[t]
     within(got, want, tol, "logits")
@@ -47,7 +47,7 @@ def test_near_and_far_rows_together(rows, cols, t, masked):
 
 
 def test_a_far_row_costs_what_a_near_one_does():
-    """Summed by each of a row's blocks it took fifty times as long."""
+    """Summed by each of a row's blocks alone it took fifty times as long."""
     x = normal(gen(1), 1, 1000000)
     target = torch.zeros(1, device="cuda", dtype=torch.int32)
     one = torch.ones(1, device="cuda")
