@@ -13,7 +13,7 @@
 // (then z = xs_i ws_j sum_k x_ik w_jk).  Products accumulate in f32 in tensor
 // memory, f32 results in pieces (PIECE); bias, activation, product and residual
 // are f32 and the result is rounded once.  dz (dg, du) is rounded to the
-// operands' type once, because the two products that follow take it as an
+// operands' type once (not for a few rows, dense_rows.cu), because the two products that follow take it as an
 // operand and kind::f16 has no wider one: against 64 bits the gradients of a
 // gated product are off by 0.0023 norm-wise in bf16, where the results' own
 // rounding is 0.0017.
@@ -1406,6 +1406,23 @@ int check_act16(bgnn_ctx* ctx, int act) {
   return BGNN_OK;
 }
 
+// what the gradients of few rows share
+RowsArgs rows_backward(const void* grad, uint64_t ld_grad, const void* x, uint64_t ld_x, uint64_t m,
+                       uint32_t k, uint32_t n, int bias_type, int act, double act_param) {
+  RowsArgs a = {};
+  a.x = x;
+  a.ld_x = ld_x;
+  a.m = (uint32_t)m;
+  a.k = k;
+  a.n = n;
+  a.bias_type = bias_type;
+  a.act = act;
+  a.act_p = (float)act_param;
+  a.grad = grad;
+  a.ld_grad = ld_grad;
+  return a;
+}
+
 // the checks that the four entry points share
 int check_product(bgnn_ctx* ctx, const char* name, int type, bool scales, const void* x,
                   uint64_t ld_x, const void* w0, uint64_t ld_w0, const void* w1, uint64_t ld_w1,
@@ -1517,6 +1534,14 @@ extern "C" int bgnn_linear_fused_backward(bgnn_ctx* ctx, int type, const void* g
     if (grad_x && m && k) BGNN_CUDA(ctx, cudaMemsetAsync(grad_x, 0, m * k * 2, ctx->stream));
     return BGNN_OK;
   }
+  if (act != BGNN_ACT_NONE && m && few_rows_backward(m, k)) {
+    RowsArgs a = rows_backward(grad, ld_grad, x, ld_x, m, k, n, bias_type, act, act_param);
+    a.w[0] = w;
+    a.ld_w[0] = ld_w;
+    a.bias[0] = bias;
+    return bgnn_run_dense_rows_backward(ctx, type, a,
+                                        {grad_x, {grad_w, nullptr}, {grad_bias, nullptr}});
+  }
   const uint32_t ldz = (n + 7) / 8 * 8;
   Mat dz[2] = {{grad, m, n, ld_grad}, {}};
   DevTmp tz, tg;
@@ -1581,6 +1606,18 @@ extern "C" int bgnn_gated_linear_backward(bgnn_ctx* ctx, int type, const void* g
   if (n == 0) {
     if (grad_x && m && k) BGNN_CUDA(ctx, cudaMemsetAsync(grad_x, 0, m * k * 2, ctx->stream));
     return BGNN_OK;
+  }
+  if (m && few_rows_backward(m, k)) {
+    RowsArgs a = rows_backward(grad, ld_grad, x, ld_x, m, k, n, bias_type, act, act_param);
+    a.two = 1;
+    a.w[0] = w_gate;
+    a.w[1] = w_up;
+    a.ld_w[0] = ld_gate;
+    a.ld_w[1] = ld_up;
+    a.bias[0] = bias_gate;
+    a.bias[1] = bias_up;
+    return bgnn_run_dense_rows_backward(
+        ctx, type, a, {grad_x, {grad_w_gate, grad_w_up}, {grad_bias_gate, grad_bias_up}});
   }
   const uint32_t ldz = (n + 7) / 8 * 8;
   DevTmp tz;  // dg, du, then the bias gradients' sums of 32 rows

@@ -14,6 +14,16 @@ inline bool few_rows(uint64_t m, uint64_t k, uint64_t n, bool two) {
   return m <= FEW_ROWS || (m * n <= SMALL_OUT && m * n * k * (two ? 2 : 1) <= SMALL_MACS);
 }
 
+// The gradients of so few rows that dz can stay in f32 (bf16, with an activation
+// and a bias, against the tensor cores, which take dz rounded): 1 x 1,024 -> 512
+// 18 us against 40, 4 x 4,096 -> 4,096 57 against 79, 8 x 256 -> 32,000 79
+// against 208; but 8 x 4,096 -> 4,096 107 against 79, 8 x 16,384 -> 256 118
+// against 108.
+constexpr uint32_t FEW_BACKWARD = 4, NARROW = 512;
+inline bool few_rows_backward(uint64_t m, uint64_t k) {
+  return m <= FEW_BACKWARD || (m <= FEW_ROWS && k <= NARROW);
+}
+
 struct RowsArgs {
   const void* x;
   uint64_t ld_x;
@@ -33,6 +43,19 @@ struct RowsArgs {
   int out_type;
   void* out;
   uint64_t ld_out;
+  const void* grad;  // backward: the upstream gradient [m, n]
+  uint64_t ld_grad;
+  float* dz[2];      // backward: dz, or dg and du, [m, n] each
 };
 // where few_rows says so; m, n >= 1
 int bgnn_run_dense_rows(bgnn_ctx* ctx, int type, const RowsArgs& a);
+
+// where few_rows_backward says so: the gradients (m, n >= 1) of a product with an
+// activation, or of a gated one; a.out, a.other and the scales are not used.
+// Any of the results may be NULL.
+struct RowsGrads {
+  void* x;       // [m, k]
+  void* w[2];    // [n, k]
+  void* bias[2]; // [n], a.bias_type
+};
+int bgnn_run_dense_rows_backward(bgnn_ctx* ctx, int type, RowsArgs a, const RowsGrads& out);

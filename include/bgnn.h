@@ -606,9 +606,10 @@ BGNN_API int bgnn_linear_fused(bgnn_ctx* ctx, int type, const void* x, uint64_t 
                                void* out, uint64_t ld_out);
 /* Its gradients for an upstream gradient grad [m, n] (type bf16 or f16, as x
  * and w): with z = x w^T + bias computed once more and dz = grad act'(z)
- * rounded to `type`, grad_x = dz w, grad_w = dz^T x (both in `type`),
- * grad_bias = column sums of the unrounded dz (bias_type).  The residual's gradient is grad.
- * Any of the three may be NULL.  Sums run in a fixed order. */
+ * rounded to `type` (kept in f32 for few rows: four, or eight of k <= 512),
+ * grad_x = dz w, grad_w = dz^T x (both in `type`), grad_bias = column sums of
+ * the unrounded dz (bias_type).  The residual's gradient is grad.  Any of the
+ * three may be NULL.  Sums run in a fixed order. */
 BGNN_API int bgnn_linear_fused_backward(bgnn_ctx* ctx, int type, const void* grad,
                                         uint64_t ld_grad, const void* x, uint64_t ld_x,
                                         const void* w, uint64_t ld_w, uint64_t m, uint32_t k,
@@ -625,7 +626,7 @@ BGNN_API int bgnn_gated_linear(bgnn_ctx* ctx, int type, const void* x, uint64_t 
                                int bias_type, const void* bias_gate, const void* bias_up, int act,
                                double act_param, int out_type, void* out, uint64_t ld_out);
 /* Its gradients: both products once more, dg = grad u act'(zg) and
- * du = grad act(zg) rounded to `type`, grad_x = dg w_gate + du w_up,
+ * du = grad act(zg) rounded to `type` (as above), grad_x = dg w_gate + du w_up,
  * grad_w_gate = dg^T x, grad_w_up = du^T x, bias gradients the column sums.
  * Any output may be NULL (the two weight gradients together). */
 BGNN_API int bgnn_gated_linear_backward(bgnn_ctx* ctx, int type, const void* grad,
